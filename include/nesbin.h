@@ -512,6 +512,64 @@ int nb_bias_grad(uint16_t *out, const uint16_t *centered, const uint16_t *bias_n
  *   modules/binary.py:63-64 on the uniform draw (which stays torch.rand), with the tensor expression's roundings. */
 int nb_bias_noise_scale(uint16_t *x, int64_t n, nb_stream_t stream);
 
+/* ---- microscaled (MX) rows: 4- and 8-bit floating values with a power-of-two scale per 32 of them ------------------
+ * No counterpart in the reference (its real-valued layers are stock torch ops).  The real-valued end of a network of
+ * binary layers: int32 sums -> RMS norm -> 8-bit rows -> product with 4-bit weights -> logits -> a token per row.
+ *
+ * Format (OCP Microscaling Formats v1.0, MXFP4 / MXFP8 E4M3): the 32 elements 32 b .. 32 b + 31 of a row share
+ * a scale 2^(s - 127), s one byte; s = 255: the block stands for NaN.  Elements are E2M1 (NB_MX_FP4: 0, .5, 1, 1.5, 2,
+ * 3, 4, 6 and a sign; element 2 i in the low half of byte i) or E4M3 (NB_MX_FP8: up to 448, 0x7F / 0xFF NaN).  With
+ * Kp = K rounded up to a multiple of 128: codes [rows, Kp / 2] or [rows, Kp] bytes, scales [rows, Kp / 32] bytes;
+ * positions K .. Kp - 1 hold zero codes, and blocks of such positions only scale byte 0.  codes and B / A operands are
+ * 16-byte aligned, scales 4-byte aligned. */
+#define NB_TYPE_F32 0
+#define NB_TYPE_F16 1
+#define NB_TYPE_BF16 2
+#define NB_TYPE_I32 3
+#define NB_MX_FP4 0
+#define NB_MX_FP8 1
+/* nb_mx_quantize: x [rows, K] (fp32, fp16 or bf16) -> MX rows.  With amax a block's largest magnitude and emax = 2
+ * (E2M1) or 8 (E4M3): s = max(floor(log2 amax) - emax + 127, 0) (0 for a block of zeros), element = x * 2^(127 - s) rounded
+ * to the nearest code, ties to the even one, at most 6 or 448 in magnitude.  An infinity or NaN in a block: s = 255, zero
+ * codes. */
+int nb_mx_quantize(uint8_t *codes, uint8_t *scales, const void *x, int type, int format, int64_t rows, int64_t K,
+                   nb_stream_t stream);
+/* nb_mx_dequantize: MX rows -> the values they stand for, out [rows, K] in fp32, fp16 or bf16 (one rounding). */
+int nb_mx_dequantize(void *out, int type, const uint8_t *codes, const uint8_t *scales, int format, int64_t rows,
+                     int64_t K, nb_stream_t stream);
+/* nb_rms_norm_mx: h = float(x) + float(residual), rounded to the residual's type and stored in residual_out [rows, K];
+ * y = float((h * (1 / sqrt(mean of h^2 over the row + eps))) * weight), everything inside in 64 bits; y -> MX rows as
+ * nb_mx_quantize converts it.  residual and residual_out NULL: h = float(x), nothing stored.  x fp32, fp16, bf16 or
+ * int32 (a binary layer's sums); the residual has x's type, or any floating one of the three where x is int32; weight [K]
+ * any floating one.  residual_out may be residual. */
+int nb_rms_norm_mx(uint8_t *codes, uint8_t *scales, void *residual_out, const void *x, int x_type, const void *residual,
+                   int residual_type, const void *weight, int weight_type, double eps, int format, int64_t rows,
+                   int64_t K, nb_stream_t stream);
+/* nb_mx_mm_nt: C[m, n] = sum_k A[m, k] * B[n, k] over MX rows, A in either format, B in E2M1; fp32 sums, rounded once to
+ * C's type (fp32, fp16, bf16); C [M, N]. */
+int nb_mx_mm_nt(void *C, int type, const uint8_t *A, const uint8_t *A_scales, int A_format, const uint8_t *B,
+                const uint8_t *B_scales, int64_t M, int64_t N, int64_t K, nb_stream_t stream);
+
+/* ---- tokens from logits and supplied words --------------------------------------------------------------------------
+ * nb_sample_tokens: one token per row of logits [R, V] (fp32, fp16, bf16 or int32), out int32 [R].  Per row, with T the
+ * temperature and m the row's largest logit: weights w_i = exp((x_i - m) / T); NaN and -inf entries have none.  The
+ * entries in descending order (equal ones by index) are cut to the shortest of three prefixes: the first top_k (all if
+ * top_k <= 0); the shortest one whose weights add up to at least top_p times those of the first top_k (all if
+ * top_p >= 1; at least one entry); those with w_i >= min(min_p, 1).  The token is the smallest index i for which the
+ * weights kept at indices up to i add up to more than words[r] / 2^32 of all that are kept.  T <= 0: the largest
+ * entry, the first of equal ones.  A row in which nothing can be drawn gives -1.  A row's largest entry +inf: the
+ * infinities share the weight equally.
+ * Weights are held as integers (61 - ceil(log2 V) fraction bits, 52 at most), so sums do not depend on an order;
+ * weights below half a unit of that are never drawn.
+ * temperature, top_k, top_p, min_p: per-row arrays [R], or NULL for the value that follows each of them for all rows
+ * (not NaN).  1 <= V <= 2^20.  workspace: nb_sample_tokens_workspace_bytes(R, V) bytes, 16-byte aligned (NULL if 0).
+ *   stands beside nb_sample_from_words (a bit per threshold and word); no counterpart in the reference. */
+int64_t nb_sample_tokens_workspace_bytes(int64_t R, int64_t V);
+int nb_sample_tokens(int32_t *out, const void *logits, int type, const uint32_t *words, const float *temperature,
+                     double temperature_all, const int32_t *top_k, int64_t top_k_all, const float *top_p,
+                     double top_p_all, const float *min_p, double min_p_all, int64_t R, int64_t V, void *workspace,
+                     int64_t workspace_bytes, nb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@ NB_OK = 0
 NB_ERR_HIP_BASE = 1000
 
 _I64, _I32, _U32, _U64, _PTR = ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p
+_F64 = ctypes.c_double
 _GEOM = [_I32] * 6
 
 # name -> argument types (without the `_i64`/`_i32` suffix expansion); every entry returns int
@@ -80,6 +81,12 @@ _PLAIN = {
     "nb_grad_regularize": [_PTR, _PTR, ctypes.c_float, ctypes.c_float, _I64, _PTR],
     "nb_bias_grad": [_PTR, _PTR, _PTR, _I64, _I64, _PTR],
     "nb_bias_noise_scale": [_PTR, _I64, _PTR],
+    "nb_mx_quantize": [_PTR, _PTR, _PTR, _I32, _I32, _I64, _I64, _PTR],
+    "nb_mx_dequantize": [_PTR, _I32, _PTR, _PTR, _I32, _I64, _I64, _PTR],
+    "nb_rms_norm_mx": [_PTR, _PTR, _PTR, _PTR, _I32, _PTR, _I32, _PTR, _I32, _F64, _I32, _I64, _I64, _PTR],
+    "nb_mx_mm_nt": [_PTR, _I32, _PTR, _PTR, _I32, _PTR, _PTR, _I64, _I64, _I64, _PTR],
+    "nb_sample_tokens": [_PTR, _PTR, _I32, _PTR, _PTR, _F64, _PTR, _I64, _PTR, _F64, _PTR, _F64, _I64, _I64, _PTR, _I64,
+                         _PTR],
 }
 # entry points that return a size (int64) instead of a status
 _SIZES = {
@@ -88,6 +95,7 @@ _SIZES = {
     "nb_skip_table_words": [],
     "nb_flip_layer_table_words": [],
     "nb_law_workspace_bytes": [],
+    "nb_sample_tokens_workspace_bytes": [_I64, _I64],
 }
 
 

@@ -13,7 +13,8 @@ half of the reference (extensions/booleanOperations.cpp:13-15) -- non-CUDA or no
 ``RuntimeError`` instead of being read through a wrong stride.
 
 Additions that the reference lacks are grouped at the end (supplied-word / Philox sampling, the fused
-sample+popcount product with a flip base, the fused conv->threshold->pack(->pool) op).
+sample+popcount product with a flip base, the fused conv->threshold->pack(->pool) op; the real-valued end of a network:
+microscaled 4- and 8-bit rows, the norm that writes them, their product, and tokens drawn from logits).
 """
 import math
 
@@ -29,6 +30,7 @@ __all__ = [
     "bmv_act_pack", "bmv_bn_act", "ExpandedRows", "expand_rows", "bmm_nt", "FlipRows", "flip_rows_from_weights",
     "bmv_flip", "bmv_flip_act_pack", "skip_table", "flip_rows_skip", "flip_rows_layered", "layer_tables", "flip_rows_to_weights",
     "center_fitness", "grad_regularize_", "bias_grad", "sample_bits_skip", "half_draws_apply", "bias_noise_scale_", "bmv_pm1",
+    "MXRows", "mx_quantize", "mx_dequantize", "rms_norm_mx", "mx_mm_nt", "sample_tokens_from_words",
 ]
 
 
@@ -1279,4 +1281,195 @@ def weighted_sum_flip(rows, weights, zbits):
     with _on(weights):
         _lib.call("nb_flip_weighted_sum_i64", out.data_ptr(), rows.entries.data_ptr(), rows.info.data_ptr(),
                   rows.base.data_ptr(), weights.data_ptr(), rows.D, rows.R, int(zbits), rows.cap, _stream(weights))
+    return out
+
+
+# ---- the real-valued end of a network: microscaled rows, norm, product, tokens ------------------------------------
+_MX_STEP = 128                       # rows are padded to whole multiples of this many elements
+_MX_FORMATS = {"fp4": (0, 2), "fp8": (1, 1)}             # format -> (its number in the C ABI, elements per code byte)
+_MX_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: 3}
+
+
+class MXRows:
+    """Rows of 4- or 8-bit floating values with a power-of-two scale per 32 of them (OCP Microscaling: MXFP4 E2M1,
+    MXFP8 E4M3; the format is spelled out in include/nesbin.h).  With Kp = ``K`` rounded up to a multiple of 128:
+    ``codes`` uint8 [rows, Kp/2] ("fp4", element 2i in the low half of byte i) or [rows, Kp] ("fp8"), ``scales`` uint8
+    [rows, Kp/32] (scale 2**(byte - 127), 255: the block stands for NaN).  Positions K..Kp-1 must hold zero codes, and
+    scale bytes other than 255 in blocks of such positions only; :func:`mx_quantize` and :func:`rms_norm_mx` write
+    them so.  Holds the tensors it is given; nothing is laid out again."""
+
+    def __init__(self, codes, scales, K, format="fp4"):
+        if format not in _MX_FORMATS:
+            raise ValueError("format must be 'fp4' or 'fp8', got %r" % (format,))
+        _check(codes, "codes")
+        _check(scales, "scales")
+        _same_device(codes, scales)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales must be torch.uint8")
+        K = int(K)
+        assert K >= 0 and len(codes.shape) == 2 and len(scales.shape) == 2
+        padded = ceil_div(K, _MX_STEP) * _MX_STEP
+        rows = codes.size(0)
+        assert codes.size(1) == padded // _MX_FORMATS[format][1]
+        assert scales.size(0) == rows and scales.size(1) == padded // 32
+        self.codes, self.scales, self.rows, self.K, self.format = codes, scales, rows, K, format
+
+    @property
+    def shape(self):
+        return (self.rows, self.K)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _mx_alloc(rows, K, format, device):
+    if format not in _MX_FORMATS:
+        raise ValueError("format must be 'fp4' or 'fp8', got %r" % (format,))
+    padded = ceil_div(K, _MX_STEP) * _MX_STEP
+    codes = torch.empty((rows, padded // _MX_FORMATS[format][1]), dtype=torch.uint8, device=device)
+    scales = torch.empty((rows, padded // 32), dtype=torch.uint8, device=device)
+    return codes, scales
+
+
+def _mx_type(t, name, types=(torch.float32, torch.float16, torch.bfloat16)):
+    if t.dtype not in types:
+        raise TypeError("%s must be one of %s, got %r" % (name, ", ".join(map(str, types)), t.dtype))
+    return _MX_TYPES[t.dtype]
+
+
+def mx_quantize(x, format="fp4"):
+    """x [rows, K] (float32, float16 or bfloat16) -> :class:`MXRows`.  Per 32 elements the scale is the power of two
+    2**(floor(log2 amax) - emax), emax = 2 for "fp4" (E2M1) and 8 for "fp8" (E4M3); elements are rounded to the nearest
+    code, ties to even, at most 6 or 448 scales in magnitude.  A block that holds an infinity or NaN stands for NaN.  The
+    real-valued counterpart of :func:`expand_rows`."""
+    _check(x, "x")
+    assert len(x.shape) == 2
+    kind = _mx_type(x, "x")
+    rows, K = x.shape
+    codes, scales = _mx_alloc(rows, K, format, x.device)
+    with _on(x):
+        _lib.call("nb_mx_quantize", codes.data_ptr(), scales.data_ptr(), x.data_ptr(), kind, _MX_FORMATS[format][0], rows,
+                  K, _stream(x))
+    return MXRows(codes, scales, K, format)
+
+
+def mx_dequantize(rows, dtype=torch.bfloat16):
+    """The values that :class:`MXRows` stand for, [rows, K] in ``dtype`` (float32, float16 or bfloat16; one rounding, and
+    none for float32, or for bfloat16 above its subnormals)."""
+    assert isinstance(rows, MXRows)
+    out = torch.empty((rows.rows, rows.K), dtype=dtype, device=rows.device)
+    kind = _mx_type(out, "dtype")
+    with _on(out):
+        _lib.call("nb_mx_dequantize", out.data_ptr(), kind, rows.codes.data_ptr(), rows.scales.data_ptr(),
+                  _MX_FORMATS[rows.format][0], rows.rows, rows.K, _stream(out))
+    return out
+
+
+def rms_norm_mx(x, weight, residual=None, eps=1e-6, format="fp8"):
+    """RMS norm with the residual's addition, written as microscaled rows: ``(MXRows, new residual or None)``.
+
+    h = x + residual (added in float32, rounded to the residual's dtype: the new residual, and what is normalised), y =
+    h / sqrt(mean(h**2) + eps) * weight in 64 bits, rounded once to float32 and converted as :func:`mx_quantize` does.
+    x [rows, K] float32, float16, bfloat16 or int32 (a binary layer's activations, see :func:`bmv_pm1`); ``residual``
+    [rows, K] of x's dtype, or of any floating one of the three where x is int32; ``weight`` [K], any of the three."""
+    _check(x, "x")
+    _check(weight, "weight")
+    _same_device(x, weight)
+    assert len(x.shape) == 2
+    rows, K = x.shape
+    x_type = _mx_type(x, "x", tuple(_MX_TYPES))
+    w_type = _mx_type(weight, "weight")
+    assert tuple(weight.shape) == (K,)
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    out, r_ptr, o_ptr, r_type = None, None, None, 0
+    if residual is not None:
+        _check(residual, "residual")
+        _same_device(x, residual)
+        assert residual.shape == x.shape
+        r_type = _mx_type(residual, "residual")
+        if x.dtype != torch.int32 and residual.dtype != x.dtype:
+            raise TypeError("the residual of a %r input must have its dtype, got %r" % (x.dtype, residual.dtype))
+        out = torch.empty_like(residual)
+        r_ptr, o_ptr = residual.data_ptr(), out.data_ptr()
+    codes, scales = _mx_alloc(rows, K, format, x.device)
+    if rows * K > 0:
+        with _on(x):
+            _lib.call("nb_rms_norm_mx", codes.data_ptr(), scales.data_ptr(), o_ptr, x.data_ptr(), x_type, r_ptr, r_type,
+                      weight.data_ptr(), w_type, eps, _MX_FORMATS[format][0], rows, K, _stream(x))
+    return MXRows(codes, scales, K, format), out
+
+
+def mx_mm_nt(A, B, dtype=torch.float32):
+    """C[m, n] = sum_k A[m, k] * B[n, k], [M, N] in ``dtype`` (float32, float16 or bfloat16): the product of two sets of
+    microscaled rows that share K, on the matrix cores; fp32 sums, rounded once.  ``A``: :class:`MXRows` in either format,
+    ``B`` in "fp4" (a layer's weights, one row per output).  The real-valued counterpart of :func:`bmm_nt`."""
+    assert isinstance(A, MXRows) and isinstance(B, MXRows)
+    assert A.K == B.K
+    if B.format != "fp4":
+        raise NotImplementedError("the second operand must be in format 'fp4'")
+    _same_device(A, B)
+    C = torch.empty((A.rows, B.rows), dtype=dtype, device=A.device)
+    kind = _mx_type(C, "dtype")
+    if A.K == 0:
+        return C.zero_()
+    with _on(C):
+        _lib.call("nb_mx_mm_nt", C.data_ptr(), kind, A.codes.data_ptr(), A.scales.data_ptr(), _MX_FORMATS[A.format][0],
+                  B.codes.data_ptr(), B.scales.data_ptr(), A.rows, B.rows, A.K, _stream(C))
+    return C
+
+
+def _row_setting(value, name, dtype, R, device):
+    """-> (pointer or None, value for all rows)"""
+    if isinstance(value, torch.Tensor):
+        _check(value, name)
+        if value.dtype != dtype:
+            raise TypeError("%s tensor must be %r, got %r" % (name, dtype, value.dtype))
+        assert tuple(value.shape) == (R,)
+        if value.device != device:
+            raise RuntimeError("Tensors are on different devices")
+        return value.data_ptr(), 0
+    value = int(value) if dtype == torch.int32 else float(value)
+    if value != value:
+        raise ValueError("%s is NaN" % name)
+    return None, value
+
+
+def sample_tokens_from_words(logits, words, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token (class) per row of ``logits`` [R, V] (float32, float16, bfloat16, or int32: a last layer's
+    activations) from one random word per row: int32 [R], -1 where nothing can be drawn.
+
+    A row's weights are w_i = exp((x_i - max) / temperature); NaN and -inf entries are never drawn.  The entries in
+    descending order (equal ones by index) are cut to the shortest of three prefixes: the first ``top_k`` (all if
+    <= 0); the shortest whose weights add up to at least ``top_p`` of those of the first top_k (all if >= 1, never
+    none); those with w_i >= ``min_p``.  The token is the smallest index up to which the kept weights add up to more than
+    word / 2**32 of all kept ones.  ``temperature`` <= 0 takes the largest entry, the first of equal ones.
+
+    ``words`` [R]: uint32 (or int32 holding the same bit patterns), e.g. from :func:`philox_words`.  Every setting is a
+    number for all rows or a tensor [R] (float32; ``top_k`` int32).  Weights are summed as integers: the same tokens
+    on every run.  Stands beside :func:`sample_bits_from_words`, which draws bits."""
+    _check(logits, "logits")
+    _check(words, "words")
+    _same_device(logits, words)
+    assert len(logits.shape) == 2
+    R, V = logits.shape
+    assert tuple(words.shape) == (R,)
+    if words.dtype not in (torch.uint32, torch.int32):
+        raise TypeError("random words must be torch.uint32 (or int32 holding the same bit patterns)")
+    assert V >= 1, "rows without entries"
+    kind = _mx_type(logits, "logits", tuple(_MX_TYPES))
+    dev = logits.device
+    t_ptr, t = _row_setting(temperature, "temperature", torch.float32, R, dev)
+    k_ptr, k = _row_setting(top_k, "top_k", torch.int32, R, dev)
+    p_ptr, p = _row_setting(top_p, "top_p", torch.float32, R, dev)
+    m_ptr, m = _row_setting(min_p, "min_p", torch.float32, R, dev)
+    k = max(min(k, 2 ** 31 - 1), 0)
+    need = _lib.load().nb_sample_tokens_workspace_bytes(R, V)
+    work = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    out = torch.empty((R,), dtype=torch.int32, device=dev)
+    with _on(logits):
+        _lib.call("nb_sample_tokens", out.data_ptr(), logits.data_ptr(), kind, words.data_ptr(), t_ptr, t, k_ptr, k, p_ptr,
+                  p, m_ptr, m, R, V, None if work is None else work.data_ptr(), need, _stream(logits))
     return out

@@ -1,0 +1,490 @@
+"""Microscaled rows, the norm that writes them, their product and the token sampler on the GPU, against the 64-bit
+restatement in oracle/mx.py."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+IDS = ["f32", "f16", "bf16"]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available()
+    from nesgpu_amd.extensions import booleanOperations
+    return booleanOperations
+
+
+def host(t):
+    return t.double().cpu().numpy()
+
+
+def rows_of(shape, seed, dtype, spread=3.0):
+    """Values of very different size per block, blocks of zeros, exact halfway points, signed zeros."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g)
+    x *= torch.exp2((torch.randn(shape[0], -(-shape[1] // 32), generator=g) * spread).round()).repeat_interleave(32, 1)[:, :shape[1]]
+    x[:, 5::7] = torch.round(x[:, 5::7] * 4) / 4
+    if shape[1] > 70:
+        x[0, 32:64] = 0.0
+        x[0, 40] = -0.0
+    return x.to(dtype)
+
+
+def as_mx(ops, codes, scales, K, format):
+    return ops.MXRows(torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda(), K, format)
+
+
+# ---- conversion -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("format", O.FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (2, 32), (5, 33), (4, 128), (3, 136), (3, 129), (7, 1000), (33, 256)])
+def test_quantize(ops, shape, dtype, format):
+    x = rows_of(shape, 11 * shape[1] + shape[0], dtype)
+    want_c, want_s = O.quantize(host(x), format)
+    got = ops.mx_quantize(x.cuda(), format)
+    assert np.array_equal(got.scales.cpu().numpy(), want_s)
+    assert np.array_equal(got.codes.cpu().numpy(), want_c)
+    assert got.shape == shape
+    back = ops.mx_dequantize(got, torch.float32)
+    assert np.array_equal(host(back), O.decode(want_c, want_s, shape[1], format))
+
+
+@pytest.mark.parametrize("format", O.FORMATS)
+def test_quantize_extremes(ops, format):
+    """Blocks at both ends of float32, subnormal ones, and blocks with an infinity or NaN."""
+    x = torch.randn(8, 128, generator=torch.Generator().manual_seed(3))
+    x[0] *= 1e-38
+    x[1] *= 1e-42
+    x[2] = 2.0 ** -149
+    x[3, :64] = torch.finfo(torch.float32).max
+    x[3, 64:] *= 2.0 ** 125
+    x[4, 3] = float("inf")
+    x[5, 40] = float("nan")
+    x[6, 127] = -float("inf")
+    x[7, :32] = 0
+    want_c, want_s = O.quantize(x.double().numpy(), format)
+    got = ops.mx_quantize(x.cuda(), format)
+    assert np.array_equal(got.scales.cpu().numpy(), want_s)
+    assert np.array_equal(got.codes.cpu().numpy(), want_c)
+    back = host(ops.mx_dequantize(got, torch.float32))
+    assert np.array_equal(back, O.decode(want_c, want_s, 128, format), equal_nan=True)
+    assert np.isnan(back[4, :32]).all() and np.isfinite(back[4, 32:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("format", O.FORMATS)
+def test_dequantize_every_code_and_scale(ops, format, dtype):
+    n = 256 if format == "fp8" else 128
+    codes = np.tile(np.arange(n, dtype=np.uint8) if format == "fp8" else np.arange(64, dtype=np.uint8), (256, 1))
+    if format == "fp4":
+        codes = np.concatenate([codes, codes + 64, codes + 128, codes + 192], axis=1)
+    K = codes.shape[1] * (2 if format == "fp4" else 1)
+    scales = np.repeat(np.arange(256, dtype=np.uint8)[:, None], K // 32, axis=1)
+    want = torch.from_numpy(O.decode(codes, scales, K, format).astype(np.float32)).to(dtype)
+    got = ops.mx_dequantize(as_mx(ops, codes, scales, K, format), dtype).cpu()
+    assert torch.equal(torch.nan_to_num(got, nan=12345.0), torch.nan_to_num(want, nan=12345.0))
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+def test_quantize_from_unaligned_storage_and_many_rows(ops):
+    flat = torch.randn(1 + 300 * 64, generator=torch.Generator().manual_seed(9)).bfloat16().cuda()
+    x = flat[1:].view(300, 64)                              # contiguous, two bytes off
+    want_c, want_s = O.quantize(host(x), "fp4")
+    got = ops.mx_quantize(x, "fp4")
+    assert np.array_equal(got.codes.cpu().numpy(), want_c) and np.array_equal(got.scales.cpu().numpy(), want_s)
+
+
+# ---- norm -------------------------------------------------------------------------------------------------------------
+def _rounder(dtype):
+    return lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dtype).float().numpy()
+
+
+NORM_TYPES = [(torch.float32, None), (torch.float16, None), (torch.bfloat16, None), (torch.int32, None),
+              (torch.float32, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
+              (torch.int32, torch.float32), (torch.int32, torch.float16), (torch.int32, torch.bfloat16)]
+
+
+def norm_inputs(shape, x_type, r_type, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g) * torch.exp(torch.randn(shape[0], 1, generator=g))
+    x = (x * 50).round().int() if x_type == torch.int32 else x.to(x_type)
+    r = None if r_type is None else (torch.randn(shape, generator=g) * (40 if x_type == torch.int32 else 1)).to(r_type)
+    w = 1 + 0.3 * torch.randn(shape[1], generator=g)
+    return x, r, w.to(r_type or (torch.float32 if x_type == torch.int32 else x_type))
+
+
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: "-".join(str(d).replace("torch.", "") for d in t))
+@pytest.mark.parametrize("shape", [(1, 1), (5, 24), (3, 77), (9, 512), (2, 520), (4, 2048), (3, 3000), (2, 5000), (1, 8192),
+                                   (2, 9001), (2, 20000), (1, 40000)])
+def test_norm(ops, shape, types):
+    x, r, w = norm_inputs(shape, *types, seed=shape[1])
+    eps = 1e-5
+    y, new = O.rms_norm(host(x), host(w), None if r is None else host(r), eps, _rounder(types[1]) if r is not None else None)
+    for format in O.FORMATS:
+        if shape[0] * shape[1] > 20000 and format == "fp4":
+            continue
+        rows, got_r = ops.rms_norm_mx(x.cuda(), w.cuda(), None if r is None else r.cuda(), eps, format)
+        if r is None:
+            assert got_r is None
+        else:
+            assert got_r.dtype == r.dtype and np.array_equal(host(got_r), new)
+        # every step before the codes is in 64 bits with one rounding to fp32: the codes themselves are equal
+        want_c, want_s = O.quantize(y.astype(np.float64), format)
+        assert np.array_equal(rows.scales.cpu().numpy(), want_s)
+        assert np.array_equal(rows.codes.cpu().numpy(), want_c)
+
+
+def test_norm_rows_of_zeros_nan_and_infinity(ops):
+    x = torch.randn(4, 256, generator=torch.Generator().manual_seed(4))
+    x[1] = 0
+    x[2, 7] = float("nan")
+    x[3, 9] = float("inf")
+    w = torch.ones(256)
+    rows, _ = ops.rms_norm_mx(x.cuda(), w.cuda())
+    v = host(ops.mx_dequantize(rows, torch.float32))
+    assert np.isfinite(v[0]).all() and np.array_equal(v[1], np.zeros(256)) and np.isnan(v[2]).all()
+    assert np.isnan(v[3, :32]).all() and np.array_equal(v[3, 32:], np.zeros(224))       # inf * 0 and finite * 0
+
+
+def test_norm_weight_of_another_type(ops):
+    x, r, _ = norm_inputs((3, 300), torch.bfloat16, torch.bfloat16, 5)
+    w = torch.rand(300, generator=torch.Generator().manual_seed(1))
+    for dt in DTYPES:
+        wt = w.to(dt)
+        y, _ = O.rms_norm(host(x), host(wt), host(r), 1e-6, _rounder(torch.bfloat16))
+        rows, _ = ops.rms_norm_mx(x.cuda(), wt.cuda(), r.cuda())
+        assert np.array_equal(rows.codes.cpu().numpy(), O.quantize(y.astype(np.float64), "fp8")[0])
+
+
+# ---- product ----------------------------------------------------------------------------------------------------------
+def product_case(M, N, K, a_format, seed):
+    g = np.random.default_rng(seed)
+    a = g.standard_normal((M, K)) * np.exp2(g.integers(-6, 7, (M, 1))) * np.where(g.random(K) < 0.05, 20, 1)
+    b = g.standard_normal((N, K)) / 8
+    qa = ref_rows(a, a_format)
+    qb = ref_rows(b, "fp4")
+    return qa, qb
+
+
+def ref_rows(x, format):
+    """MX rows of float64 values, through torch for speed (the conversion itself is tested above)."""
+    t = O.table(format)
+    rows, K = x.shape
+    Kp = O.padded(K)
+    v = np.zeros((rows, Kp // 32, 32))
+    v.reshape(rows, Kp)[:, :K] = x
+    amax = np.abs(v).max(axis=2)
+    e = np.where(amax > 0, np.frexp(np.where(amax > 0, amax, 1))[1] - 1 - O.EMAX[format], -127).clip(-127, 127)
+    q = np.ldexp(np.abs(v), -e[:, :, None]).reshape(rows, Kp)
+    hi = np.searchsorted(t, q).clip(1, len(t) - 1)
+    c = np.where(t[hi] - q < q - t[hi - 1], hi, hi - 1)
+    c = (c + np.signbit(v.reshape(rows, Kp)) * (8 if format == "fp4" else 128)).astype(np.uint8)
+    if format == "fp4":
+        c = c[:, 0::2] | (c[:, 1::2] << 4)
+    return np.ascontiguousarray(c), (e + 127).astype(np.uint8)
+
+
+SHAPES = [(1, 1, 1), (1, 32, 128), (3, 5, 33), (16, 16, 256), (17, 33, 640), (1, 1000, 4096), (2, 640, 1111), (100, 10, 2048),
+          (64, 64, 512), (65, 130, 1000), (128, 256, 384), (200, 300, 129), (257, 513, 1280), (600, 520, 2304), (1, 7, 16384),
+          (5, 4099, 512), (300, 10, 8192), (1030, 70, 130)]
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_product(ops, shape, a_format):
+    M, N, K = shape
+    (ac, as_), (bc, bs) = product_case(M, N, K, a_format, M + 3 * N + K)
+    want, size = O.mm_nt(O.decode(ac, as_, K, a_format), O.decode(bc, bs, K, "fp4"))
+    A, B = as_mx(ops, ac, as_, K, a_format), as_mx(ops, bc, bs, K, "fp4")
+    # products are exact and every partial sum is at most `size`: one rounding (allowed to be a truncation, 2^-23) per
+    # addition into an accumulator; a step of 128 positions adds its groups of 8, and partial sums are joined at the end
+    adds = 2 * 17 * (O.padded(K) // 128) + 64
+    for dtype in DTYPES:
+        got = host(ops.mx_mm_nt(A, B, dtype))
+        half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+        bound = adds * 2.0 ** -23 * size + half * np.abs(want) + (2.0 ** -25 if dtype == torch.float16 else 0)
+        if dtype == torch.float16:
+            ok = np.abs(want) < 65000
+            assert np.all(np.abs(got - want)[ok] <= bound[ok] * (1 + half))
+        else:
+            assert np.all(np.abs(got - want) <= bound * (1 + half))
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+@pytest.mark.parametrize("shape", [(1, 64, 512), (70, 90, 256), (300, 300, 512)], ids=lambda s: "x".join(map(str, s)))
+def test_product_of_small_whole_numbers_is_exact(ops, shape, a_format):
+    M, N, K = shape
+    g = np.random.default_rng(7)
+    a, b = g.integers(-3, 4, (M, K)).astype(float), g.integers(-2, 3, (N, K)).astype(float)
+    A, B = as_mx(ops, *ref_rows(a, a_format), K, a_format), as_mx(ops, *ref_rows(b, "fp4"), K, "fp4")
+    assert np.array_equal(host(ops.mx_mm_nt(A, B)), a @ b.T)
+
+
+@pytest.mark.parametrize("shape", [(1, 32, 512), (40, 40, 256), (260, 300, 512)], ids=lambda s: "x".join(map(str, s)))
+def test_product_keeps_small_values_beside_large_ones(ops, shape):
+    """E4M3 neighbours 17 binades apart whose large products cancel: what is left is the small ones' exact sum."""
+    M, N, K = shape
+    a = np.zeros((M, K))
+    a[:, 0::8], a[:, 1::8] = 256.0, -256.0
+    g = np.random.default_rng(2)
+    a[:, 2::8] = g.integers(1, 8, (M, K // 8)) * 2.0 ** -9
+    a[:, 5::8] = g.integers(8, 16, (M, K // 8)) * 2.0 ** -9
+    b = np.ones((N, K))
+    b[:, 2::8] = g.choice([0.5, 1.5, -3.0], (N, K // 8))
+    ac, as_ = ref_rows(a, "fp8")
+    assert np.all(as_ == 127)
+    B = as_mx(ops, *ref_rows(b, "fp4"), K, "fp4")
+    got = host(ops.mx_mm_nt(as_mx(ops, ac, as_, K, "fp8"), B))
+    # the running sum passes through 256: multiples of 2^-10 below 2^9 are 19 bits, exact in fp32
+    assert np.array_equal(got, a @ b.T)
+
+
+def test_product_of_nan_blocks_and_extreme_scales(ops):
+    K = 256
+    (ac, as_), (bc, bs) = product_case(20, 24, K, "fp8", 1)
+    as_[3, 2] = 255
+    bs[5, 7] = 255
+    ac[9, 100] = 0x7F
+    got = host(ops.mx_mm_nt(as_mx(ops, ac, as_, K, "fp8"), as_mx(ops, bc, bs, K, "fp4")))
+    nan = np.zeros((20, 24), dtype=bool)
+    nan[3] = nan[9] = True
+    nan[:, 5] = True
+    assert np.array_equal(np.isnan(got), nan)
+    # scales that leave float32's range by themselves and meet inside it
+    a, b = np.ones((4, 128)), np.ones((4, 128))
+    for fmt in O.FORMATS:
+        (ac, as_), (bc, bs) = ref_rows(a, fmt), ref_rows(b, "fp4")
+        as_[:] = 250
+        bs[:] = 4
+        want = O.decode(ac, as_, 128, fmt) @ O.decode(bc, bs, 128, "fp4").T
+        assert np.array_equal(host(ops.mx_mm_nt(as_mx(ops, ac, as_, 128, fmt), as_mx(ops, bc, bs, 128, "fp4"))), want)
+
+
+# ---- tokens -----------------------------------------------------------------------------------------------------------
+def check_tokens(ops, x, words, **kw):
+    R = x.shape[0]
+    args = {k: (torch.tensor(v, dtype=torch.int32 if k == "top_k" else torch.float32).cuda() if isinstance(v, list) else v)
+            for k, v in kw.items()}
+    got = ops.sample_tokens_from_words(x.cuda(), words.cuda(), **args).cpu().tolist()
+    xs = host(x)
+    w = (words.long() & 0xFFFFFFFF).tolist()
+    f32 = {k: ([float(np.float32(e)) if k != "top_k" else e for e in v] if isinstance(v, list) else v) for k, v in kw.items()}
+    want = [O.sample(xs[r], w[r], **{k: (v[r] if isinstance(v, list) else v) for k, v in f32.items()}) for r in range(R)]
+    assert got == want
+
+
+def words_of(R, seed):
+    w = torch.randint(-2 ** 31, 2 ** 31, (R,), generator=torch.Generator().manual_seed(seed)).int()
+    if R > 3:
+        w[0], w[1] = 0, -1                                  # the smallest and the largest word
+    return w
+
+
+SETTINGS = [dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=7), dict(top_p=0.8), dict(top_p=0.3, temperature=1.5),
+            dict(min_p=0.1), dict(top_k=20, top_p=0.9, min_p=0.02, temperature=0.9), dict(temperature=0.0), dict(top_p=0.0),
+            dict(min_p=1.0), dict(min_p=5.0), dict(top_k=10 ** 9, top_p=2.0), dict(temperature=100.0, top_p=0.999)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int32], ids=IDS + ["i32"])
+@pytest.mark.parametrize("V", [1, 2, 10, 63, 64, 65, 500, 513, 2048, 2049, 5000])
+def test_tokens(ops, V, dtype):
+    g = torch.Generator().manual_seed(V)
+    R = 12 if V < 1000 else 5
+    x = torch.randn(R, V, generator=g) * 2.5
+    x = (x * 3).round().int() if dtype == torch.int32 else x.to(dtype)
+    if dtype != torch.int32 and V > 4:
+        x[:, ::5] = -float("inf")
+        x[2, 1::3] = float("nan")
+        x[3] = -float("inf")
+    for n, kw in enumerate(SETTINGS):
+        check_tokens(ops, x, words_of(R, n), **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int32], ids=["bf16", "i32"])
+def test_tokens_of_long_rows(ops, dtype):
+    g = torch.Generator().manual_seed(77)
+    for V in (16384, 16385, 40001, 131072):
+        x = torch.randn(2, V, generator=g) * 2.5
+        x = (x * 20).round().int() if dtype == torch.int32 else x.to(dtype)
+        for n, kw in enumerate([dict(temperature=10.0 if dtype == torch.int32 else 1.0, top_p=0.9), dict(top_k=50),
+                                dict(top_k=5000, top_p=0.95, min_p=1e-4, temperature=1.3), dict()]):
+            check_tokens(ops, x, words_of(2, n), **kw)
+
+
+def test_tokens_with_settings_per_row(ops):
+    g = torch.Generator().manual_seed(5)
+    R, V = 40, 700
+    x = torch.randn(R, V, generator=g) * 3
+    kw = dict(temperature=(torch.rand(R, generator=g) * 2).tolist(), top_k=torch.randint(-1, 60, (R,), generator=g).tolist(),
+              top_p=(torch.rand(R, generator=g) * 1.2).tolist(), min_p=(torch.rand(R, generator=g) * 0.2).tolist())
+    kw["temperature"][4] = 0.0
+    kw["temperature"][5] = -1.0
+    check_tokens(ops, x, words_of(R, 8), **kw)
+
+
+@pytest.mark.parametrize("V", [40, 3000, 40000])
+def test_tokens_of_equal_entries(ops, V):
+    """Every border falls among equal entries: ties are kept by index, sums of equal weights are exact."""
+    for dtype in (torch.float32, torch.float16, torch.int32):
+        x = torch.zeros(6, V)
+        x[2, : V // 2] = -1.0
+        x[3, V // 2] = -0.0
+        x = x.to(dtype)
+        for kw in (dict(top_k=3), dict(top_p=0.5), dict(top_k=V // 2, top_p=0.5), dict(), dict(temperature=0.0)):
+            check_tokens(ops, x, words_of(6, 1), **kw)
+
+
+def test_tokens_with_infinities_and_extremes(ops):
+    inf = float("inf")
+    x = torch.tensor([[0.0, inf, 1.0, inf], [-inf, -inf, -inf, -inf], [-inf, 3e38, -3e38, 3e38], [float("nan"), -inf, -5.0, inf],
+                      [float("nan")] * 4, [1e-45, 0.0, -0.0, -1e-45]])
+    for kw in (dict(), dict(top_k=1), dict(top_p=0.4), dict(temperature=0.0), dict(temperature=float("inf")),
+               dict(temperature=1e-30), dict(min_p=0.5), dict(temperature=1e30, top_k=2)):
+        if kw.get("temperature") == inf:
+            got = ops.sample_tokens_from_words(x.cuda(), words_of(6, 2).cuda(), **kw).cpu()
+            assert got[1] == -1 and got[4] == -1 and (got[[0, 2, 3, 5]] >= 0).all()
+            continue
+        check_tokens(ops, x, words_of(6, 2), **kw)
+    big = torch.tensor([[-2 ** 31, 2 ** 31 - 1, 0, 2 ** 31 - 1], [-2 ** 31] * 4, [-2 ** 31, -2 ** 31 + 1, 7, 8]], dtype=torch.int32)
+    for kw in (dict(), dict(top_k=3), dict(top_p=0.9, temperature=1e9), dict(temperature=0.0)):
+        check_tokens(ops, big, words_of(3, 3), **kw)
+
+
+def test_tokens_follow_their_weights(ops):
+    """Over evenly spread words every token comes as often as its weight says, to one word."""
+    p = np.array([0.4, 0.3, 0.2, 0.05, 0.05])
+    n = 4096
+    x = torch.tensor(np.log(p), dtype=torch.float32).repeat(n, 1)
+    words = ((torch.arange(n, dtype=torch.int64) << 20) + (1 << 19)).to(torch.uint32)
+    got = ops.sample_tokens_from_words(x.cuda(), words.cuda()).cpu()
+    assert np.all(np.abs(np.bincount(got.numpy(), minlength=5) - p * n) <= 1.01)
+
+
+# ---- refusals and the run of them together ------------------------------------------------------------------------------
+def test_refusals(ops):
+    x = torch.zeros(4, 64, device="cuda")
+    w = torch.zeros(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.mx_quantize(x[:, ::2])
+    with pytest.raises(TypeError):
+        ops.mx_quantize(x.double())
+    with pytest.raises(ValueError):
+        ops.mx_quantize(x, "fp6")
+    with pytest.raises(AssertionError):
+        ops.rms_norm_mx(x, torch.ones(63, device="cuda"))
+    with pytest.raises(TypeError):
+        ops.rms_norm_mx(x, torch.ones(64, device="cuda"), x.half())
+    with pytest.raises(ValueError):
+        ops.rms_norm_mx(x, torch.ones(64, device="cuda"), eps=-1.0)
+    q4, q8 = ops.mx_quantize(x), ops.mx_quantize(x, "fp8")
+    with pytest.raises(NotImplementedError):
+        ops.mx_mm_nt(q4, q8)
+    with pytest.raises(AssertionError):
+        ops.mx_mm_nt(q4, ops.mx_quantize(x[:, :32].contiguous()))
+    with pytest.raises(TypeError):
+        ops.mx_mm_nt(q4, q4, torch.float64)
+    with pytest.raises(AssertionError):
+        ops.MXRows(q4.codes, q4.scales, 200)
+    with pytest.raises(AssertionError):
+        ops.sample_tokens_from_words(x, w[:3])
+    with pytest.raises(TypeError):
+        ops.sample_tokens_from_words(x, w.long())
+    with pytest.raises(TypeError):
+        ops.sample_tokens_from_words(x, w, temperature=torch.ones(4, device="cuda", dtype=torch.float64))
+    with pytest.raises(ValueError):
+        ops.sample_tokens_from_words(x, w, top_p=float("nan"))
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.sample_tokens_from_words(torch.zeros(1, (1 << 20) + 1, device="cuda"), w[:1].clone())
+
+
+def test_empty_inputs(ops):
+    e = torch.zeros(0, 64, device="cuda")
+    q = ops.mx_quantize(e)
+    assert q.shape == (0, 64) and ops.mx_dequantize(q).shape == (0, 64)
+    assert ops.mx_mm_nt(q, ops.mx_quantize(torch.ones(3, 64, device="cuda"))).shape == (0, 3)
+    z = ops.mx_quantize(torch.zeros(3, 0, device="cuda"))
+    assert torch.equal(ops.mx_mm_nt(z, z), torch.zeros(3, 3, device="cuda"))
+    assert ops.rms_norm_mx(e, torch.ones(64, device="cuda"), e)[1].shape == (0, 64)
+    assert ops.sample_tokens_from_words(e, torch.zeros(0, dtype=torch.int32, device="cuda")).shape == (0,)
+
+
+def head(ops, act, stream, gain, weights, words, **kw):
+    rows, stream = ops.rms_norm_mx(act, gain, stream, eps=1e-5)
+    logits = ops.mx_mm_nt(rows, weights, torch.float32)
+    return ops.sample_tokens_from_words(logits, words, **kw), stream, logits
+
+
+def test_from_binary_layer_to_token(ops):
+    """A binary layer's int32 activations and a residual stream -> norm -> readout -> a class per member, each step against
+    the oracle on the step's own input."""
+    from nesgpu_amd.modules import binary
+    D, K, N = 96, 512, 37
+    torch.manual_seed(3)
+    layer = binary.BinarizedLinear(256, K, D, threshold=False)
+    with torch.no_grad():
+        layer.weight.copy_(torch.randn(K, 256))
+    model = binary.PerturbedModel(layer, D)
+    model.set_seed(5)
+    model.set_noise(1.0)
+    bits = torch.rand(D, 256, device="cuda") < 0.5
+    act = model.forward(bits)
+    assert act.dtype == torch.int32 and tuple(act.shape) == (D, K)
+    stream = (torch.randn(D, K, device="cuda") * 10).half()
+    gain = 1 + 0.1 * torch.randn(K, device="cuda")
+    weights = ops.mx_quantize(torch.randn(N, K, device="cuda"), "fp4")
+    words = ops.philox_words(D, 11)
+    kw = dict(temperature=8.0, top_k=20, top_p=0.9)
+    token, new, logits = head(ops, act, stream, gain, weights, words, **kw)
+    y, want_new = O.rms_norm(host(act), host(gain), host(stream), 1e-5, _rounder(torch.float16))
+    assert np.array_equal(host(new), want_new)
+    qc, qs = O.quantize(y.astype(np.float64), "fp8")
+    a = O.decode(qc, qs, K, "fp8")
+    b = O.decode(weights.codes.cpu().numpy(), weights.scales.cpu().numpy(), K, "fp4")
+    want, size = O.mm_nt(a, b)
+    assert np.all(np.abs(host(logits) - want) <= (2 * 17 * 4 + 64) * 2.0 ** -23 * size)
+    w = (words.cpu().to(torch.int64) & 0xFFFFFFFF).tolist()
+    assert token.cpu().tolist() == [O.sample(host(logits)[d], w[d], **kw) for d in range(D)]
+
+
+def test_captured_and_on_another_stream(ops):
+    """The run of them in a graph, replayed on new inputs with eager work between, equals the eager run; so does a run on a
+    side stream."""
+    D, K, N = 40, 300, 5000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    gain = torch.ones(K, device="cuda")
+    weights = ops.mx_quantize(torch.randn(N, K, generator=g, device="cuda"), "fp4")
+    kw = dict(temperature=2.0, top_p=0.9)
+
+    def inputs():
+        return (torch.randint(-200, 200, (D, K), generator=g, device="cuda").int(),
+                torch.randn(D, K, generator=g, device="cuda").bfloat16(),
+                torch.randint(-2 ** 31, 2 ** 31, (D,), generator=g, device="cuda").int())
+
+    act, stream, words = inputs()
+    head(ops, act, stream, gain, weights, words, **kw)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                                       # two graphs, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = head(ops, act, stream, gain, weights, words, **kw)
+        graphs.append((graph, out))
+    for k in range(4):
+        new = inputs()
+        for t, n in zip((act, stream, words), new):
+            t.copy_(n)
+        want = head(ops, *new[:2], gain, weights, new[2], **kw)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = head(ops, *new[:2], gain, weights, new[2], **kw)
+        torch.cuda.current_stream().wait_stream(side)
+        graph, out = graphs[k % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(want, out, other):
+            assert torch.equal(a, b) and torch.equal(a, c)

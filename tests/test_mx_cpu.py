@@ -1,0 +1,124 @@
+"""Microscaled rows, norm, product and token sampler without a GPU: the oracle's own pins, and what is refused before
+anything is launched."""
+import ctypes
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from nesgpu_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__ as g
+        g.build()
+    return _lib.load()
+
+
+# ---- oracle pins ----------------------------------------------------------------------------------------------------
+def test_tables():
+    assert O.table("fp4").max() == 6 and O.table("fp8").max() == 448 and len(O.table("fp8")) == 127
+    f8 = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(O.table("fp8"), f8)
+
+
+@pytest.mark.parametrize("format", O.FORMATS)
+def test_values_of_the_format_are_kept(format):
+    t = O.table(format)
+    x = np.zeros((1, 256))
+    x[0, :len(t)] = t
+    x[0, 128:128 + len(t)] = -t
+    x[0, 0::32] = t[-1]                                    # every block reaches the largest value: scale 1
+    c, s = O.quantize(x, format)
+    assert np.all(s == 127)
+    assert np.array_equal(O.decode(c, s, 256, format), x)
+
+
+@pytest.mark.parametrize("format", O.FORMATS)
+def test_error_is_at_most_half_a_step(format):
+    g = np.random.default_rng(1)
+    x = g.standard_normal((4, 320)) * np.exp(g.standard_normal((4, 1)) * 5)
+    c, s = O.quantize(x, format)
+    v = O.decode(c, s, 320, format)
+    half = {"fp4": 2.0 ** -2, "fp8": 2.0 ** -4}[format]    # of the value's own binade ...
+    scale = np.ldexp(1.0, np.repeat(s.astype(int), 32, axis=1)[:, :320] - 127)
+    smallest = {"fp4": 0.25, "fp8": 2.0 ** -10}[format]    # ... or half the smallest code
+    top = O.table(format)[-1] * scale
+    inside = np.abs(x) <= top
+    assert np.all(np.abs(v - x)[inside] <= np.maximum(half * np.abs(x), smallest * scale)[inside])
+    assert np.array_equal(np.abs(v)[~inside], top[~inside])              # saturated
+
+
+def test_sampler_keeps_the_shortest_prefix():
+    x = np.log([0.5, 0.25, 0.125, 0.125])
+    # words spread over the unit interval: the shares of what is kept
+    def shares(**kw):
+        got = [O.sample(x, int(u * 2 ** 32), **kw) for u in (np.arange(64) + 0.5) / 64]
+        return [got.count(i) for i in range(4)]
+    assert shares() == [32, 16, 8, 8]
+    assert shares(top_k=1) == [64, 0, 0, 0] and shares(top_k=3)[3] == 0
+    assert shares(top_p=0.74)[2:] == [0, 0]
+    assert shares(min_p=0.3)[2:] == [0, 0]
+    assert shares(temperature=0.0) == [64, 0, 0, 0]
+    assert O.sample(np.full(5, -np.inf), 7) == -1
+    assert O.sample(np.array([np.nan, 1.0, -np.inf]), 2 ** 32 - 1) == 1
+    assert [O.sample(np.zeros(4), w, top_p=0.5) for w in (0, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1)] == [0, 0, 1, 1]
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+def test_c_abi_refuses_before_launching(lib):
+    one, odd = ctypes.c_void_p(256), ctypes.c_void_p(257)
+    err = lib.nb_last_error_string
+    assert lib.nb_mx_quantize(one, one, one, 0, 0, -1, 32, None) == 2
+    assert lib.nb_mx_quantize(one, one, one, 3, 0, 1, 32, None) == 2 and b"type" in err()
+    assert lib.nb_mx_quantize(one, one, one, 0, 2, 1, 32, None) == 2 and b"format" in err()
+    assert lib.nb_mx_quantize(None, one, one, 0, 0, 1, 32, None) == 1
+    assert lib.nb_mx_quantize(odd, one, one, 0, 0, 1, 32, None) == 3
+    assert lib.nb_mx_quantize(one, one, odd, 1, 0, 1, 32, None) == 3
+    assert lib.nb_mx_quantize(one, one, one, 0, 0, 1 << 39, 1 << 39, None) == 2
+    assert lib.nb_mx_quantize(None, None, None, 0, 0, 0, 32, None) == 0              # nothing to do
+    assert lib.nb_mx_dequantize(one, 3, one, one, 0, 1, 32, None) == 2
+    assert lib.nb_mx_dequantize(one, 0, one, None, 0, 1, 32, None) == 1
+    # norm: a residual of another floating type, half a pair, a negative eps
+    assert lib.nb_rms_norm_mx(one, one, one, one, 2, one, 0, one, 0, 1e-6, 1, 1, 32, None) == 2 and b"residual" in err()
+    assert lib.nb_rms_norm_mx(one, one, None, one, 2, one, 2, one, 0, 1e-6, 1, 1, 32, None) == 1
+    assert lib.nb_rms_norm_mx(one, one, None, one, 2, None, 0, one, 0, -1.0, 1, 1, 32, None) == 2
+    assert lib.nb_rms_norm_mx(one, one, None, one, 2, None, 0, one, 0, float("nan"), 1, 1, 32, None) == 2
+    assert lib.nb_rms_norm_mx(one, one, None, one, 2, None, 0, one, 3, 1e-6, 1, 1, 32, None) == 2
+    # product: no inner length, an output type, formats
+    assert lib.nb_mx_mm_nt(one, 0, one, one, 0, one, one, 1, 1, 0, None) == 2
+    assert lib.nb_mx_mm_nt(one, 3, one, one, 0, one, one, 1, 1, 32, None) == 2
+    assert lib.nb_mx_mm_nt(one, 0, one, one, 5, one, one, 1, 1, 32, None) == 2
+    assert lib.nb_mx_mm_nt(one, 0, one, odd, 0, one, one, 1, 1, 32, None) == 3
+    assert lib.nb_mx_mm_nt(None, 0, None, None, 0, None, None, 0, 5, 32, None) == 0
+    # tokens
+    args = (None, 1.0, None, 0, None, 1.0, None, 0.0)
+    assert lib.nb_sample_tokens(one, one, 0, one, *args, 1, 0, None, 0, None) == 2
+    assert lib.nb_sample_tokens(one, one, 0, one, *args, 1, (1 << 20) + 1, None, 0, None) == 2
+    assert lib.nb_sample_tokens(one, one, 4, one, *args, 1, 8, None, 0, None) == 2
+    assert lib.nb_sample_tokens(one, None, 0, one, *args, 1, 8, None, 0, None) == 1
+    assert lib.nb_sample_tokens(one, odd, 0, one, *args, 1, 8, None, 0, None) == 3
+    assert lib.nb_sample_tokens(one, one, 0, one, None, math.nan, *args[2:], 1, 8, None, 0, None) == 2
+    assert lib.nb_sample_tokens(None, None, 0, None, *args, 0, 8, None, 0, None) == 0
+
+
+def test_python_refuses_host_tensors():
+    from nesgpu_amd.extensions import booleanOperations as ops
+    x = torch.zeros(2, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.mx_quantize(x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.rms_norm_mx(x, torch.ones(64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.sample_tokens_from_words(x, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.MXRows(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(2, 4, dtype=torch.uint8), 64)
+    with pytest.raises(ValueError, match="format"):
+        ops.MXRows(x, x, 64, "fp6")
