@@ -9,54 +9,60 @@
 // they reach the fp32 accumulator: exact for E2M1 x E2M1 (products are multiples of 1/4 up to 36) but not for E4M3, whose
 // values span 18 binades: a product 2^-14 of its neighbour is lost (relative error of a sum of normal values 4e-6, with
 // a few columns 20 times larger 2e-5, measured over K = 8192).  The E4M3 operand is therefore split in two whose
-// products fit: values of magnitude 4 and more (multiples of 1/2 up to 448) and smaller ones (multiples of 2^-9); two
-// instructions per step, every sum exact to fp32.
+// products fit: values of magnitude 2 and more (multiples of 1/4 up to 448) and smaller ones (multiples of 2^-9); two
+// instructions per step, every sum exact to fp32 (no difference in 10^5 dense sums of random and extreme codes of
+// either part).
 #include <algorithm>
+#include <atomic>
+#include <cmath>
 
 #include "nb_mx.hpp"
 
 namespace nb {
 
-// Bytes of E4M3 codes with magnitude >= 4 (code 0x48) as a mask; NaN (0x7F) among them.
+// Bytes of E4M3 codes with magnitude >= 2 (the exponent's top bit) as a mask; NaN (0x7F) among them.
 __device__ __forceinline__ uint32_t mx_large_mask(uint32_t a)
 {
-    const uint32_t h = ((a & 0x7F7F7F7Fu) + 0x38383838u) & 0x80808080u;   // no carry between bytes: 0x7F + 0x38 < 0x100
-    return (h << 1) - (h >> 7);
+    const uint32_t h = a & 0x40404040u;
+    return (h << 2) - (h >> 6);
 }
 
+// an E2M1 fragment as the instruction's operand (its upper half is not read)
+__device__ __forceinline__ mx_v8i mx_wide(mx_v4i b) { return __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1); }
+__device__ __forceinline__ mx_v8i mx_frag4(const uint8_t *p) { return mx_wide(*reinterpret_cast<const mx_v4i *>(p)); }
+
+// The products of one step: E2M1 as it is, E4M3 in its two parts (smaller values first)
 template <bool FP8>
-struct MxA;
-template <>
-struct MxA<false> {
-    mx_v8i v;
-    __device__ __forceinline__ void load(const uint8_t *row, int g)
-    {
-        const mx_v4i a = *reinterpret_cast<const mx_v4i *>(row + 16 * g);
-        v = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
-    }
-};
-template <>
-struct MxA<true> {
-    mx_v8i v;
-    __device__ __forceinline__ void load(const uint8_t *row, int g)
-    {
-        const mx_v4i a = *reinterpret_cast<const mx_v4i *>(row + 16 * g);
-        const mx_v4i b = *reinterpret_cast<const mx_v4i *>(row + 64 + 16 * g);
-        v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-};
-
-__device__ __forceinline__ mx_v8i mx_frag4(const uint8_t *p)
+__device__ __forceinline__ void mx_step(mx_v4f &acc, const mx_v8i &lo, const mx_v8i &hi, const mx_v8i &b, int sa, int sb)
 {
-    const mx_v4i b = *reinterpret_cast<const mx_v4i *>(p);
-    return __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
+    if constexpr (FP8) {
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(lo, b, acc, 0, 4, 0, sa, 0, sb);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hi, b, acc, 0, 4, 0, sa, 0, sb);
+    } else {
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hi, b, acc, 4, 4, 0, sa, 0, sb);
+    }
+}
+template <bool FP8>
+__device__ __forceinline__ void mx_split(mx_v8i &lo, mx_v8i &hi, mx_v4i a0, mx_v4i a1)
+{
+    if constexpr (FP8) {
+        const mx_v8i a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t m = mx_large_mask((uint32_t)a[e]);
+            hi[e] = (int)((uint32_t)a[e] & m);
+            lo[e] = (int)((uint32_t)a[e] & ~m);
+        }
+    } else {
+        hi = mx_wide(a0);
+    }
 }
 
-template <typename O>
-__device__ __forceinline__ void mx_store_out(O *c, float v) { mx_store1(c, v); }
-
-// A workgroup makes one tile of 16 MT x 16 NT outputs; its W waves take every W-th step of K, fragments straight
-// from memory, and their sums meet in shared memory in a fixed order.
+// ---- few rows: one operand is streamed, fragments straight from memory ------------------------------------------------
+// A workgroup makes one tile of 16 MT x 16 NT outputs; its W waves take every W-th chunk of four steps, and their sums
+// meet in shared memory in a fixed order.  What bounds it is the number of row pieces per load, about 4 cycles each
+// whatever their size: a fragment load has 16 of 64 bytes, and a load of one scale dword per row would cost as much again,
+// so a row's four scale dwords of a chunk come in one load (where they are aligned; else one by one).
 template <bool FP8, typename O, int MT, int NT, int W>
 __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, const uint8_t *__restrict__ A,
                                                             const uint32_t *__restrict__ As, const uint8_t *__restrict__ B,
@@ -86,37 +92,52 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = mx_v4f{0.f, 0.f, 0.f, 0.f};
-    for (int64_t s = wave; s < steps; s += W) {
-        mx_v8i fb[NT];
-        int sb[NT];
+    const bool whole = (steps & 3) == 0;
+    const auto scales4 = [&](const uint32_t *p) {
+        if (whole) return *reinterpret_cast<const mx_v4i *>(p);
+        return mx_v4i{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+    };
+    const int64_t chunks = steps >> 2;
+    for (int64_t c = wave; c < chunks; c += W) {
+        mx_v4i fb[NT][4], fa[MT][4][FP8 ? 2 : 1], sb[NT], sa[MT];
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            fb[j] = mx_frag4(b[j] + s * 64 + 16 * g);
-            sb[j] = (int)(bs[j][s] >> (8 * g));
+#pragma unroll
+            for (int e = 0; e < 4; e++) fb[j][e] = *reinterpret_cast<const mx_v4i *>(b[j] + (4 * c + e) * 64 + 16 * g);
+            sb[j] = scales4(bs[j] + 4 * c);
         }
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            MxA<FP8> fa;
-            fa.load(a[i] + s * ABYTES, g);
-            const int sa = (int)(as[i][s] >> (8 * g));
-            if (FP8) {
-                mx_v8i hi, lo;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t m = mx_large_mask((uint32_t)fa.v[e]);
-                    hi[e] = (int)((uint32_t)fa.v[e] & m);
-                    lo[e] = (int)((uint32_t)fa.v[e] & ~m);
-                }
+            for (int e = 0; e < 4; e++) {
+                const uint8_t *p = a[i] + (4 * c + e) * ABYTES + 16 * g;
+                fa[i][e][0] = *reinterpret_cast<const mx_v4i *>(p);
+                if (FP8) fa[i][e][FP8 ? 1 : 0] = *reinterpret_cast<const mx_v4i *>(p + 64);
+            }
+            sa[i] = scales4(as[i] + 4 * c);
+        }
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(lo, fb[j], acc[i][j], 0, 4, 0, sa, 0, sb[j]);
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hi, fb[j], acc[i][j], 0, 4, 0, sa, 0, sb[j]);
-                }
-            } else {
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                mx_v8i lo, hi;
+                mx_split<FP8>(lo, hi, fa[i][e][0], fa[i][e][FP8 ? 1 : 0]);
 #pragma unroll
                 for (int j = 0; j < NT; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa.v, fb[j], acc[i][j], 4, 4, 0, sa, 0, sb[j]);
+                    mx_step<FP8>(acc[i][j], lo, hi, mx_wide(fb[j][e]), (int)((uint32_t)sa[i][e] >> (8 * g)),
+                                 (int)((uint32_t)sb[j][e] >> (8 * g)));
             }
+    }
+    for (int64_t s = 4 * chunks + wave; s < steps; s += W) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const uint8_t *p = a[i] + s * ABYTES + 16 * g;
+            mx_v8i lo, hi;
+            mx_split<FP8>(lo, hi, *reinterpret_cast<const mx_v4i *>(p), *reinterpret_cast<const mx_v4i *>(p + (FP8 ? 64 : 0)));
+            const int sa = (int)(as[i][s] >> (8 * g));
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                mx_step<FP8>(acc[i][j], lo, hi, mx_frag4(b[j] + s * 64 + 16 * g), sa, (int)(bs[j][s] >> (8 * g)));
         }
     }
 #pragma unroll
@@ -132,8 +153,258 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
         for (int w = 0; w < W; w++) v += part[w][t >> 8][t & 255];
         const int64_t m = 16 * (mt * MT + (t >> 8) / NT) + ((t & 255) >> 4);
         const int64_t n = 16 * (nt * NT + (t >> 8) % NT) + (t & 15);
-        if (m < M && n < N) mx_store_out(C + m * N + n, v);
+        if (m < M && n < N) mx_store1(C + m * N + n, v);
     }
+}
+
+// ---- tiles staged through LDS ----------------------------------------------------------------------------------------
+// A workgroup of WM x WN waves makes a tile of 16 MT WM x 16 NT WN outputs.  A step of 128 positions of its rows goes from
+// memory to LDS without passing registers (16 bytes per lane), two steps ahead of the products: three buffers, one
+// barrier per step.  LDS rows are as dense as in memory (64 bytes of E2M1, 128 of E4M3, which is what such a
+// load writes); the 16-byte pieces of a row are permuted by the row's number, at the source address and again where
+// fragments are read, so that the 16 rows of a fragment read lie in different banks.  Scales come four steps at a time,
+// 16 bytes per row.
+template <int BYTES>
+__device__ __forceinline__ int mx_swizzle(int row)
+{
+    // A 16-byte read by 64 lanes runs in four turns of 16 lanes over the 64 banks (256 bytes).  A turn holds all 16 rows
+    // of a fragment, rows 0-3 and 12-15 of one piece number with rows 4-11 of the next (or all of one): with the piece
+    // numbers XORed as below its 16 pieces fill the banks in either case.  Measured: no conflicts left, where
+    // permutations for 32 banks or turns of neighbouring lanes cost half as many cycles again.
+    const int q = (row >> 2) & 3;
+    return BYTES == 64 ? (((q ^ (q >> 1)) & 1) << 1) | (q >> 1) : (row >> 1) & 7;
+}
+
+typedef __attribute__((address_space(3))) void *mx_lds_ptr;
+typedef const __attribute__((address_space(1))) void *mx_global_ptr;
+__device__ __forceinline__ void mx_to_lds16(const void *g, void *l)
+{
+    __builtin_amdgcn_global_load_lds((mx_global_ptr)g, (mx_lds_ptr)l, 16, 0, 0);
+}
+__device__ __forceinline__ void mx_to_lds4(const void *g, void *l)
+{
+    __builtin_amdgcn_global_load_lds((mx_global_ptr)g, (mx_lds_ptr)l, 4, 0, 0);
+}
+// All but the latest N loads of this wave have arrived, and what it read from LDS is in registers.
+template <int N>
+__device__ __forceinline__ void mx_wait_loads()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
+}
+
+__device__ __forceinline__ void mx_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+template <bool FP8, int WM, int WN, int MT, int NT, int BUFFERS>
+struct MxTile {
+    static constexpr int WAVES = WM * WN, TM = 16 * MT * WM, TN = 16 * NT * WN;
+    static constexpr int ABYTES = FP8 ? 128 : 64;
+    static constexpr int kStage = TM * ABYTES + TN * 64, kBuffers = BUFFERS, kAhead = BUFFERS - 1;   // stages ahead
+    static constexpr int kScales = (TM + TN) * 16;                       // four steps
+    static constexpr int kLds = kBuffers * kStage + 2 * kScales;
+    // A stage comes in 1 KB pieces (a wave's 64 lanes of 16 bytes), the scales in pieces of 64 rows.  Every wave asks for
+    // the same number of them, so that its count of loads is known; where there are fewer pieces than that, some waves
+    // ask for the first ones again.
+    static constexpr int A_PIECES = TM * ABYTES / 1024, B_PIECES = TN * 64 / 1024, S_PIECES = (TM + TN) / 64;
+    static constexpr int A_LOADS = (A_PIECES + WAVES - 1) / WAVES, B_LOADS = (B_PIECES + WAVES - 1) / WAVES;
+    static constexpr int S_LOADS = (S_PIECES + WAVES - 1) / WAVES;
+    static constexpr int LOADS = A_LOADS + B_LOADS;
+    // All but so many loads have arrived when stage s + 1 has, behind the loads of step s (the next group's scales and
+    // stage s + kAhead).  Where the scales lie among the later loads they are allowed for only if that is the newest stage:
+    // for more stages ahead the wait is then S_LOADS loads stricter than it need be, once in four steps.
+    static constexpr int wait(bool group) { return (kAhead - 1) * LOADS + (kAhead == 2 && group ? S_LOADS : 0); }
+    // the waits below: a group of scales, asked for four steps before its first use, has arrived with all but the latest
+    // kAhead - 1 stages
+    static_assert(kAhead >= 2 && kAhead <= 5, "stages ahead");
+    static_assert(TM % 64 == 0 && TN % 64 == 0 && kLds <= 160 * 1024, "LDS");
+    static constexpr int64_t kMaxSteps = (1LL << 31) / (TM > TN ? TM : TN) / ABYTES - 1;   // 32-bit offsets
+};
+
+template <bool FP8, typename O, int WM, int WN, int MT, int NT, int BUFFERS>
+__global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict__ C, const uint8_t *__restrict__ A,
+                                                                  const uint32_t *__restrict__ As,
+                                                                  const uint8_t *__restrict__ B,
+                                                                  const uint32_t *__restrict__ Bs, int M, int N,
+                                                                  int steps, int mtiles, int ntiles)
+{
+    using P = MxTile<FP8, WM, WN, MT, NT, BUFFERS>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+    // workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in strips of 8 tiles of M
+    const int T = mtiles * ntiles, per = (T + 7) / 8;
+    const int L = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    if (L >= T) return;                                                  // the whole workgroup, before any barrier
+    constexpr int kStrip = 8;
+    const int strip = L / (kStrip * ntiles), in = L - strip * kStrip * ntiles;
+    const int height = mtiles - strip * kStrip < kStrip ? mtiles - strip * kStrip : kStrip;
+    const int mt = strip * kStrip + in % height, nt = in / height;
+    const int m0 = mt * P::TM, n0 = nt * P::TN;
+
+    // this lane's loads, as offsets from the tile's first row (below 2^31: the host sends no longer rows here); rows past
+    // the end read the last row again and are not stored
+    const uint8_t *const a_tile = A + (int64_t)m0 * steps * P::ABYTES, *const b_tile = B + (int64_t)n0 * steps * 64;
+    const int a_last = M - 1 - m0, b_last = N - 1 - n0;
+    uint32_t a_src[P::A_LOADS], b_src[P::B_LOADS], s_src[P::S_LOADS];
+#pragma unroll
+    for (int q = 0; q < P::A_LOADS; q++) {
+        constexpr int lanes = P::ABYTES / 16;                            // lanes per row
+        const int row = (q * P::WAVES + wave) % P::A_PIECES * (64 / lanes) + lane / lanes;
+        a_src[q] = (uint32_t)((row < a_last ? row : a_last) * steps * P::ABYTES +
+                              16 * ((lane % lanes) ^ mx_swizzle<P::ABYTES>(row)));
+    }
+#pragma unroll
+    for (int q = 0; q < P::B_LOADS; q++) {
+        const int row = (q * P::WAVES + wave) % P::B_PIECES * 16 + lane / 4;
+        b_src[q] = (uint32_t)((row < b_last ? row : b_last) * steps * 64 + 16 * ((lane % 4) ^ mx_swizzle<64>(row)));
+    }
+    const uint32_t *const as_tile = As + (int64_t)m0 * steps, *const bs_tile = Bs + (int64_t)n0 * steps;
+#pragma unroll
+    for (int q = 0; q < P::S_LOADS; q++) {
+        // 64 rows of one operand (TM is a multiple of 64), the same one for the whole wave
+        const int row0 = (q * P::WAVES + wave) % P::S_PIECES * 64, row = (row0 < P::TM ? row0 : row0 - P::TM) + lane;
+        const int last = row0 < P::TM ? a_last : b_last;
+        s_src[q] = (uint32_t)((row < last ? row : last) * steps) * 4;
+    }
+    uint8_t *const scales = lds + P::kBuffers * P::kStage;
+    // steps % 4 == 0: a row's four dwords at once, [row][4]; else one by one, [step][row]
+    const bool whole = (steps & 3) == 0;
+    const int s_row = whole ? 16 : 4, s_step = whole ? 4 : 4 * (P::TM + P::TN);
+    const auto load_scales = [&](int group) {
+        uint8_t *to = scales + (group & 1) * P::kScales;
+        const int at = 4 * group < steps ? 4 * group : 0;
+#pragma unroll
+        for (int q = 0; q < P::S_LOADS; q++) {
+            const int row0 = (q * P::WAVES + wave) % P::S_PIECES * 64;
+            const uint8_t *from = reinterpret_cast<const uint8_t *>(row0 < P::TM ? as_tile : bs_tile);
+            if (whole) {
+                mx_to_lds16(from + 4 * at + s_src[q], to + row0 * 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    mx_to_lds4(from + 4 * (at + j < steps ? at + j : steps - 1) + s_src[q],
+                               to + j * 4 * (P::TM + P::TN) + row0 * 4);
+            }
+        }
+    };
+    const auto load_stage = [&](int s) {
+        uint8_t *to = lds + (s % P::kBuffers) * P::kStage;
+        const int at = s < steps ? s : steps - 1;                        // past the end: the same number of loads
+#pragma unroll
+        for (int q = 0; q < P::A_LOADS; q++)
+            mx_to_lds16(a_tile + at * P::ABYTES + a_src[q], to + (q * P::WAVES + wave) % P::A_PIECES * 1024);
+#pragma unroll
+        for (int q = 0; q < P::B_LOADS; q++)
+            mx_to_lds16(b_tile + at * 64 + b_src[q], to + P::TM * P::ABYTES + (q * P::WAVES + wave) % P::B_PIECES * 1024);
+    };
+    mx_v4f acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = mx_v4f{0.f, 0.f, 0.f, 0.f};
+    const int a_row = wm * MT * 16 + r16, b_row = wn * NT * 16 + r16;
+    const int a_off0 = a_row * P::ABYTES + 16 * (g ^ mx_swizzle<P::ABYTES>(r16));
+    const int a_off1 = a_row * P::ABYTES + 16 * ((g + 4) ^ mx_swizzle<P::ABYTES>(r16));
+    const int b_off = P::TM * P::ABYTES + b_row * 64 + 16 * (g ^ mx_swizzle<64>(r16));
+    mx_v4i fa[MT][FP8 ? 2 : 1], fb[NT];
+    int sa[MT], sb[NT];
+    const auto fetch = [&](int s) {
+        const uint8_t *buf = lds + (s % P::kBuffers) * P::kStage;
+        const uint8_t *sc = scales + ((s >> 2) & 1) * P::kScales + (s & 3) * s_step;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            fb[j] = *reinterpret_cast<const mx_v4i *>(buf + b_off + j * 16 * 64);
+            sb[j] = (int)(*reinterpret_cast<const uint32_t *>(sc + (P::TM + b_row + 16 * j) * s_row) >> (8 * g));
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            sa[i] = (int)(*reinterpret_cast<const uint32_t *>(sc + (a_row + 16 * i) * s_row) >> (8 * g));
+            fa[i][0] = *reinterpret_cast<const mx_v4i *>(buf + a_off0 + i * 16 * P::ABYTES);
+            if constexpr (FP8) fa[i][1] = *reinterpret_cast<const mx_v4i *>(buf + a_off1 + i * 16 * P::ABYTES);
+        }
+    };
+    const auto multiply = [&]() {
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            mx_v8i lo, hi;
+            mx_split<FP8>(lo, hi, fa[i][0], fa[i][FP8 ? 1 : 0]);
+            if constexpr (FP8) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(lo, mx_wide(fb[j]), acc[i][j], 0, 4, 0, sa[i], 0, sb[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hi, mx_wide(fb[j]), acc[i][j], FP8 ? 0 : 4, 4, 0, sa[i], 0, sb[j]);
+        }
+    };
+    load_scales(0);
+#pragma unroll
+    for (int t = 0; t < P::kAhead; t++) load_stage(t);
+    if constexpr (P::WAVES == 8) {
+        // Two waves per SIMD, one of each half of the workgroup, half a step apart: while one half reads its fragments
+        // the other multiplies.  A phase ends with a barrier; half 0 reads step s in phase 2 s and multiplies in phase
+        // 2 s + 1, half 1 a phase later.  The stage asked for in the phase that reads step s goes to the buffer that held
+        // stage s - 1, which both halves have read by the end of phase 2 s - 1.  Stage s + 1 has to be there at the
+        // end of phase 2 s + 1, where half 0 has multiplied step s and half 1 has read it.
+        const bool half1 = wave >= 4;
+        mx_wait_loads<P::wait(false)>();
+        __builtin_amdgcn_s_barrier();
+        if (half1) __builtin_amdgcn_s_barrier();
+        for (int s = 0; s < steps; s++) {
+            const bool group = (s & 3) == 0;
+            if (group) load_scales((s >> 2) + 1);
+            load_stage(s + P::kAhead);
+            fetch(s);
+            if (half1) {
+                if (group) mx_wait_loads<P::wait(true)>();
+                else mx_wait_loads<P::wait(false)>();
+            } else {
+                mx_wait_lds();
+            }
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_s_setprio(1);
+            multiply();
+            // the products belong to this phase (nothing else keeps them on this side of the barrier)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) asm volatile("" : "+v"(acc[i][j]));
+            __builtin_amdgcn_s_setprio(0);
+            if (!half1) {
+                if (group) mx_wait_loads<P::wait(true)>();
+                else mx_wait_loads<P::wait(false)>();
+            }
+            __builtin_amdgcn_s_barrier();
+        }
+        if (!half1) __builtin_amdgcn_s_barrier();
+    } else {
+        // Step s: stage s has arrived, for this wave (the wait) and for all (the barrier), behind which all waves are also
+        // done with the buffer of stage s - 1, which takes the next one.  Other workgroups of the CU fill the waits.
+        mx_wait_loads<P::wait(false)>();
+        for (int s = 0; s < steps; s++) {
+            const bool group = (s & 3) == 0;
+            __builtin_amdgcn_s_barrier();
+            if (group) load_scales((s >> 2) + 1);
+            load_stage(s + P::kAhead);
+            fetch(s);
+            multiply();
+            if (group) mx_wait_loads<P::wait(true)>();
+            else mx_wait_loads<P::wait(false)>();
+        }
+    }
+    mx_wait_loads<0>();                  // nothing is on its way to LDS when the workgroup ends
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int m = m0 + (wm * MT + i) * 16 + 4 * g + r;
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int n = n0 + (wn * NT + j) * 16 + r16;
+                if (m < M && n < N) mx_store1(C + (int64_t)m * N + n, acc[i][j][r]);
+            }
+        }
 }
 
 struct MmArgs {
@@ -144,15 +415,88 @@ struct MmArgs {
     hipStream_t st;
 };
 
-template <bool FP8, typename O>
-static int mm_launch(const MmArgs &a, const char *who)
+template <bool FP8, typename O, int WM, int WN, int MT, int NT, int BUFFERS>
+static int mm_tile_launch(const MmArgs &a, const char *who)
 {
-    constexpr int MT = 1, NT = 2, W = 4;
+    using P = MxTile<FP8, WM, WN, MT, NT, BUFFERS>;
+    const int64_t mt = ceil_div(a.M, P::TM), nt = ceil_div(a.N, P::TN);
+    NB_REQUIRE(mt * nt < (1 << 21) && a.steps <= P::kMaxSteps, "%s: too many tiles", who);
+    auto *kernel = mx_mm_tile_kernel<FP8, O, WM, WN, MT, NT, BUFFERS>;
+    static std::atomic<uint64_t> ready{0};              // devices on which the kernel's LDS size has been set
+    int device = 0;
+    (void)hipGetDevice(&device);
+    if (device < 0 || device > 63 || !(ready.load() >> device & 1)) {
+        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::kLds);
+        if (e != hipSuccess) return fail(NB_ERR_HIP_BASE + (int)e, "%s: %s", who, hipGetErrorString(e));
+        if (device >= 0 && device <= 63) ready.fetch_or(1ull << device);
+    }
+    kernel<<<dim3((unsigned)(ceil_div(mt * nt, 8) * 8)), dim3(64 * WM * WN), P::kLds, a.st>>>(
+        (O *)a.C, a.A, a.As, a.B, a.Bs, (int)a.M, (int)a.N, (int)a.steps, (int)mt, (int)nt);
+    return check_launch(who);
+}
+
+template <bool FP8, typename O, int MT, int NT, int W>
+static int mm_rows_launch(const MmArgs &a, const char *who)
+{
     const int64_t mt = ceil_div(a.M, 16 * MT), nt = ceil_div(a.N, 16 * NT);
-    NB_REQUIRE(mt * nt < (1LL << 31) / (64 * W) * 2, "%s: too many tiles", who);
+    NB_REQUIRE(mt * nt < (1LL << 32) / (64 * W), "%s: too many tiles", who);
     mx_mm_rows_kernel<FP8, O, MT, NT, W><<<dim3((unsigned)(mt * nt)), dim3(64 * W), 0, a.st>>>(
         (O *)a.C, a.A, a.As, a.B, a.Bs, a.M, a.N, a.steps, nt);
     return check_launch(who);
+}
+
+// Which kernel: the one whose time is least by two measured costs, in microseconds per step of K: `alone` where every CU
+// has at most one workgroup (a step's latency), `full` for 256 workgroups of a launch that fills the card many times over.
+// Measured at K = 8192, in microseconds, E4M3 / E2M1:
+//                        256x256      128x128     64x128      64x64       16x64       16x32       16x16
+//   4096 x 16384        702 / 275    902 / 373   961 / 517  1070 / 716
+//   4096 x 1024         165 /  64     77 /  34    63 /  37    72 /  48
+//   1024 x 1024         163 /  63     75 /  32    42 /  23    29 /  18
+//     64 x 8192                                   42 /  23    29 /  19    30 /  25    36 /  28
+//     16 x 32768                                  45 /  24    43 /  24    31 /  26    38 /  31    52 / -
+//      1 x 32768                                  45 /  24    42 /  23    28 /  24    33 /  28    34 / 32
+//      1 x 8192                                   41 /  22    29 /  18    16 /  13     9 /   8
+struct MmCost {
+    int rows, columns;
+    bool one_per_cu;      // a CU holds one workgroup: what fills the card comes in whole rounds of 256
+    double alone, full;
+};
+constexpr MmCost kMmCosts[2][7] = {
+    // E2M1 x E2M1
+    {{256, 256, true, 0.97, 1.07}, {128, 128, false, 0.50, 0.364}, {64, 128, false, 0.34, 0.253}, {64, 64, false, 0.27, 0.173},
+     {16, 64, false, 0.20, 0.18}, {16, 32, false, 0.10, 0.10}, {16, 16, false, 0.055, 0.055}},
+    // E4M3 x E2M1
+    {{256, 256, true, 2.55, 2.74}, {128, 128, false, 1.15, 0.88}, {64, 128, false, 0.62, 0.469}, {64, 64, false, 0.45, 0.261},
+     {16, 64, false, 0.25, 0.22}, {16, 32, false, 0.14, 0.13}, {16, 16, false, 0.07, 0.06}},
+};
+
+static int mm_choice(const MmArgs &a, bool fp8)
+{
+    int best = 0;
+    double least = 0;
+    for (int v = 0; v < 7; v++) {
+        if (v < 4 && a.steps > 65536) continue;                  // longer rows than the tiles' offsets reach
+        const MmCost &c = kMmCosts[fp8][v];
+        double rounds = (double)ceil_div(a.M, c.rows) * (double)ceil_div(a.N, c.columns) / 256.0;
+        if (c.one_per_cu) rounds = ceil(rounds);
+        const double cost = std::max(c.alone, c.full * rounds);
+        if (least == 0 || cost < least) best = v, least = cost;
+    }
+    return best;
+}
+
+template <bool FP8, typename O>
+static int mm_launch(const MmArgs &a, const char *who)
+{
+    switch (mm_choice(a, FP8)) {
+        case 0: return mm_tile_launch<FP8, O, 4, 2, 4, 8, FP8 ? 3 : 4>(a, who);
+        case 1: return mm_tile_launch<FP8, O, 2, 2, 4, 4, 3>(a, who);
+        case 2: return mm_tile_launch<FP8, O, 2, 2, 2, 4, 4>(a, who);
+        case 3: return mm_tile_launch<FP8, O, 4, 1, 1, 4, 4>(a, who);
+        case 4: return mm_rows_launch<FP8, O, 1, 4, 4>(a, who);
+        case 5: return mm_rows_launch<FP8, O, 1, 2, 4>(a, who);
+        default: return mm_rows_launch<FP8, O, 1, 1, 8>(a, who);
+    }
 }
 
 }  // namespace nb
@@ -165,7 +509,7 @@ int nb_mx_mm_nt(void *C, int type, const uint8_t *A, const uint8_t *A_scales, in
     NB_REQUIRE(M >= 0 && N >= 0 && K >= 1, "%s: bad shape", who);
     NB_REQUIRE(type >= NB_TYPE_F32 && type <= NB_TYPE_BF16, "%s: type %d", who, type);
     NB_REQUIRE(A_format == NB_MX_FP4 || A_format == NB_MX_FP8, "%s: format %d", who, A_format);
-    NB_REQUIRE(M < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31), "%s: too large", who);
+    NB_REQUIRE(M <= (1LL << 30) && N <= (1LL << 30) && K <= (1LL << 30), "%s: too large", who);
     if (M * N == 0) return NB_OK;
     NB_REQUIRE_PTR(C);
     NB_REQUIRE_PTR(A);

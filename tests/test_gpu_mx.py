@@ -214,6 +214,32 @@ def test_product(ops, shape, a_format):
             assert np.all(np.abs(got - want) <= bound * (1 + half))
 
 
+# sizes at which each of the kernels is the cheapest (tiles of 256x256, 128x128, 64x128, 64x64; 16 rows by 64, 32, 16), K of one
+# step, of whole groups of four steps and of odd ones
+LARGE = [(8100, 8191, 1100), (8192, 8192, 128), (8000, 8300, 512), (3000, 3000, 700), (2048, 2100, 1536), (2049, 2100, 200),
+         (2000, 1100, 900), (1030, 1025, 2048), (1000, 1000, 1000), (20, 33000, 640), (7, 40000, 1150), (40, 8000, 3000),
+         (1, 3000, 6000), (2000, 20, 2100), (3, 129, 33000)]
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+@pytest.mark.parametrize("shape", LARGE, ids=lambda s: "x".join(map(str, s)))
+def test_product_of_large_sizes(ops, shape, a_format):
+    M, N, K = shape
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    a = torch.randn(M, K, generator=g, device="cuda") * torch.exp2(torch.randint(-6, 7, (M, 1), generator=g, device="cuda"))
+    a[:, ::19] *= 20
+    A = ops.mx_quantize(a, a_format)
+    B = ops.mx_quantize(torch.randn(N, K, generator=g, device="cuda") / 8, "fp4")
+    a, b = ops.mx_dequantize(A, torch.float32).double(), ops.mx_dequantize(B, torch.float32).double()
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    adds = 2 * 17 * (O.padded(K) // 128) + 64                # as in test_product
+    for dtype in (torch.float32, torch.bfloat16):
+        got = ops.mx_mm_nt(A, B, dtype).double()
+        half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+        err = (got - want).abs() - (adds * 2.0 ** -23 * size + half * want.abs()) * (1 + half)
+        assert float(err.max()) <= 0
+
+
 @pytest.mark.parametrize("a_format", O.FORMATS)
 @pytest.mark.parametrize("shape", [(1, 64, 512), (70, 90, 256), (300, 300, 512)], ids=lambda s: "x".join(map(str, s)))
 def test_product_of_small_whole_numbers_is_exact(ops, shape, a_format):
