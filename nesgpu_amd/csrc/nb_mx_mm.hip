@@ -67,7 +67,7 @@ template <bool FP8, typename O, int MT, int NT, int W>
 __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, const uint8_t *__restrict__ A,
                                                             const uint32_t *__restrict__ As, const uint8_t *__restrict__ B,
                                                             const uint32_t *__restrict__ Bs, int64_t M, int64_t N,
-                                                            int64_t steps, int64_t ntiles)
+                                                            int64_t steps, int64_t ntiles, bool whole)
 {
     constexpr int ABYTES = FP8 ? 128 : 64;
     __shared__ float part[W][MT * NT][256];
@@ -92,7 +92,6 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = mx_v4f{0.f, 0.f, 0.f, 0.f};
-    const bool whole = (steps & 3) == 0;
     const auto scales4 = [&](const uint32_t *p) {
         if (whole) return *reinterpret_cast<const mx_v4i *>(p);
         return mx_v4i{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
@@ -224,7 +223,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
                                                                   const uint32_t *__restrict__ As,
                                                                   const uint8_t *__restrict__ B,
                                                                   const uint32_t *__restrict__ Bs, int M, int N,
-                                                                  int steps, int mtiles, int ntiles)
+                                                                  int steps, int mtiles, int ntiles, bool whole)
 {
     using P = MxTile<FP8, WM, WN, MT, NT, BUFFERS>;
     extern __shared__ __align__(16) uint8_t lds[];
@@ -267,8 +266,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
         s_src[q] = (uint32_t)((row < last ? row : last) * steps) * 4;
     }
     uint8_t *const scales = lds + P::kBuffers * P::kStage;
-    // steps % 4 == 0: a row's four dwords at once, [row][4]; else one by one, [step][row]
-    const bool whole = (steps & 3) == 0;
+    // a row's four dwords at once, [row][4], or one by one, [step][row]
     const int s_row = whole ? 16 : 4, s_step = whole ? 4 : 4 * (P::TM + P::TN);
     const auto load_scales = [&](int group) {
         uint8_t *to = scales + (group & 1) * P::kScales;
@@ -412,6 +410,7 @@ struct MmArgs {
     const uint8_t *A, *B;
     const uint32_t *As, *Bs;
     int64_t M, N, steps;
+    bool whole;           // four steps' scales of a row are 16 aligned bytes
     hipStream_t st;
 };
 
@@ -431,7 +430,7 @@ static int mm_tile_launch(const MmArgs &a, const char *who)
         if (device >= 0 && device <= 63) ready.fetch_or(1ull << device);
     }
     kernel<<<dim3((unsigned)(ceil_div(mt * nt, 8) * 8)), dim3(64 * WM * WN), P::kLds, a.st>>>(
-        (O *)a.C, a.A, a.As, a.B, a.Bs, (int)a.M, (int)a.N, (int)a.steps, (int)mt, (int)nt);
+        (O *)a.C, a.A, a.As, a.B, a.Bs, (int)a.M, (int)a.N, (int)a.steps, (int)mt, (int)nt, a.whole);
     return check_launch(who);
 }
 
@@ -441,7 +440,7 @@ static int mm_rows_launch(const MmArgs &a, const char *who)
     const int64_t mt = ceil_div(a.M, 16 * MT), nt = ceil_div(a.N, 16 * NT);
     NB_REQUIRE(mt * nt < (1LL << 32) / (64 * W), "%s: too many tiles", who);
     mx_mm_rows_kernel<FP8, O, MT, NT, W><<<dim3((unsigned)(mt * nt)), dim3(64 * W), 0, a.st>>>(
-        (O *)a.C, a.A, a.As, a.B, a.Bs, a.M, a.N, a.steps, nt);
+        (O *)a.C, a.A, a.As, a.B, a.Bs, a.M, a.N, a.steps, nt, a.whole);
     return check_launch(who);
 }
 
@@ -521,8 +520,10 @@ int nb_mx_mm_nt(void *C, int type, const uint8_t *A, const uint8_t *A_scales, in
     NB_REQUIRE_ALIGNED(B, 16);
     NB_REQUIRE_ALIGNED(A_scales, 4);
     NB_REQUIRE_ALIGNED(B_scales, 4);
+    const int64_t steps = nb::mx_padded(K) / nb::kMxStep;
     const nb::MmArgs a{C, A, B, reinterpret_cast<const uint32_t *>(A_scales), reinterpret_cast<const uint32_t *>(B_scales),
-                       M, N, nb::mx_padded(K) / nb::kMxStep, nb::as_stream(stream)};
+                       M, N, steps, steps % 4 == 0 && nb::aligned(A_scales, 16) && nb::aligned(B_scales, 16),
+                       nb::as_stream(stream)};
     const bool fp8 = A_format == NB_MX_FP8;
     if (type == NB_TYPE_F32) return fp8 ? nb::mm_launch<true, float>(a, who) : nb::mm_launch<false, float>(a, who);
     if (type == NB_TYPE_F16) return fp8 ? nb::mm_launch<true, _Float16>(a, who) : nb::mm_launch<false, _Float16>(a, who);

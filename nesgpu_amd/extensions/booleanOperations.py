@@ -1295,8 +1295,10 @@ class MXRows:
     MXFP8 E4M3; the format is spelled out in include/nesbin.h).  With Kp = ``K`` rounded up to a multiple of 128:
     ``codes`` uint8 [rows, Kp/2] ("fp4", element 2i in the low half of byte i) or [rows, Kp] ("fp8"), ``scales`` uint8
     [rows, Kp/32] (scale 2**(byte - 127), 255: the block stands for NaN).  Positions K..Kp-1 must hold zero codes, and
-    scale bytes other than 255 in blocks of such positions only; :func:`mx_quantize` and :func:`rms_norm_mx` write
-    them so.  Holds the tensors it is given; nothing is laid out again."""
+    blocks of such positions only no scale byte 255; :func:`mx_quantize` and :func:`rms_norm_mx` write
+    them so.  Holds the tensors it is given (both start 16 and 4 bytes aligned); nothing is laid out again."""
+
+    __slots__ = ("_codes", "_scales", "_code_bytes", "_device", "rows", "K", "format")
 
     def __init__(self, codes, scales, K, format="fp4"):
         if format not in _MX_FORMATS:
@@ -1307,12 +1309,48 @@ class MXRows:
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("codes and scales must be torch.uint8")
         K = int(K)
-        assert K >= 0 and len(codes.shape) == 2 and len(scales.shape) == 2
+        assert len(codes.shape) == 2
+        rows, code_bytes = codes.shape
         padded = ceil_div(K, _MX_STEP) * _MX_STEP
-        rows = codes.size(0)
-        assert codes.size(1) == padded // _MX_FORMATS[format][1]
-        assert scales.size(0) == rows and scales.size(1) == padded // 32
-        self.codes, self.scales, self.rows, self.K, self.format = codes, scales, rows, K, format
+        assert K >= 0 and code_bytes == padded // _MX_FORMATS[format][1]
+        assert tuple(scales.shape) == (rows, padded // 32)
+        self._codes, self._scales, self._code_bytes, self._device = codes, scales, code_bytes, codes.device
+        self.rows, self.K, self.format = rows, K, format
+
+    @classmethod
+    def _empty(cls, rows, K, format, device):
+        """Rows to be written by a kernel: codes and scales in one allocation, as tensors of their own when asked for."""
+        if format not in _MX_FORMATS:
+            raise ValueError("format must be 'fp4' or 'fp8', got %r" % (format,))
+        padded = ceil_div(K, _MX_STEP) * _MX_STEP
+        self = cls.__new__(cls)
+        self._code_bytes = padded // _MX_FORMATS[format][1]
+        self._codes = None
+        self._scales = torch.empty((rows * (self._code_bytes + padded // 32),), dtype=torch.uint8, device=device)
+        self._device = device
+        self.rows, self.K, self.format = rows, K, format
+        return self
+
+    def _pointers(self):
+        if self._codes is None:
+            both = self._scales.data_ptr()
+            return both, both + self.rows * self._code_bytes
+        return self._codes.data_ptr(), self._scales.data_ptr()
+
+    def _parts(self):
+        if self._codes is None:
+            both, n = self._scales, self.rows * self._code_bytes
+            self._codes = both[:n].view(self.rows, self._code_bytes)
+            self._scales = both[n:].view(self.rows, -1) if self.rows else both.view(0, ceil_div(self.K, _MX_STEP) * 4)
+        return self._codes, self._scales
+
+    @property
+    def codes(self):
+        return self._parts()[0]
+
+    @property
+    def scales(self):
+        return self._parts()[1]
 
     @property
     def shape(self):
@@ -1320,16 +1358,7 @@ class MXRows:
 
     @property
     def device(self):
-        return self.codes.device
-
-
-def _mx_alloc(rows, K, format, device):
-    if format not in _MX_FORMATS:
-        raise ValueError("format must be 'fp4' or 'fp8', got %r" % (format,))
-    padded = ceil_div(K, _MX_STEP) * _MX_STEP
-    codes = torch.empty((rows, padded // _MX_FORMATS[format][1]), dtype=torch.uint8, device=device)
-    scales = torch.empty((rows, padded // 32), dtype=torch.uint8, device=device)
-    return codes, scales
+        return self._device
 
 
 def _mx_type(t, name, types=(torch.float32, torch.float16, torch.bfloat16)):
@@ -1347,11 +1376,11 @@ def mx_quantize(x, format="fp4"):
     assert len(x.shape) == 2
     kind = _mx_type(x, "x")
     rows, K = x.shape
-    codes, scales = _mx_alloc(rows, K, format, x.device)
+    out = MXRows._empty(rows, K, format, x.device)
     with _on(x):
-        _lib.call("nb_mx_quantize", codes.data_ptr(), scales.data_ptr(), x.data_ptr(), kind, _MX_FORMATS[format][0], rows,
-                  K, _stream(x))
-    return MXRows(codes, scales, K, format)
+        _lib.call("nb_mx_quantize", *out._pointers(), x.data_ptr(), kind, _MX_FORMATS[format][0], rows, K,
+                  _stream(x))
+    return out
 
 
 def mx_dequantize(rows, dtype=torch.bfloat16):
@@ -1361,7 +1390,7 @@ def mx_dequantize(rows, dtype=torch.bfloat16):
     out = torch.empty((rows.rows, rows.K), dtype=dtype, device=rows.device)
     kind = _mx_type(out, "dtype")
     with _on(out):
-        _lib.call("nb_mx_dequantize", out.data_ptr(), kind, rows.codes.data_ptr(), rows.scales.data_ptr(),
+        _lib.call("nb_mx_dequantize", out.data_ptr(), kind, *rows._pointers(),
                   _MX_FORMATS[rows.format][0], rows.rows, rows.K, _stream(out))
     return out
 
@@ -1394,12 +1423,12 @@ def rms_norm_mx(x, weight, residual=None, eps=1e-6, format="fp8"):
             raise TypeError("the residual of a %r input must have its dtype, got %r" % (x.dtype, residual.dtype))
         out = torch.empty_like(residual)
         r_ptr, o_ptr = residual.data_ptr(), out.data_ptr()
-    codes, scales = _mx_alloc(rows, K, format, x.device)
+    y = MXRows._empty(rows, K, format, x.device)
     if rows * K > 0:
         with _on(x):
-            _lib.call("nb_rms_norm_mx", codes.data_ptr(), scales.data_ptr(), o_ptr, x.data_ptr(), x_type, r_ptr, r_type,
+            _lib.call("nb_rms_norm_mx", *y._pointers(), o_ptr, x.data_ptr(), x_type, r_ptr, r_type,
                       weight.data_ptr(), w_type, eps, _MX_FORMATS[format][0], rows, K, _stream(x))
-    return MXRows(codes, scales, K, format), out
+    return y, out
 
 
 def mx_mm_nt(A, B, dtype=torch.float32):
@@ -1416,8 +1445,8 @@ def mx_mm_nt(A, B, dtype=torch.float32):
     if A.K == 0:
         return C.zero_()
     with _on(C):
-        _lib.call("nb_mx_mm_nt", C.data_ptr(), kind, A.codes.data_ptr(), A.scales.data_ptr(), _MX_FORMATS[A.format][0],
-                  B.codes.data_ptr(), B.scales.data_ptr(), A.rows, B.rows, A.K, _stream(C))
+        _lib.call("nb_mx_mm_nt", C.data_ptr(), kind, *A._pointers(), _MX_FORMATS[A.format][0],
+                  *B._pointers(), A.rows, B.rows, A.K, _stream(C))
     return C
 
 
