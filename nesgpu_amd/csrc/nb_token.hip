@@ -10,13 +10,14 @@
 // however few the rows), one workgroup per row to finish from the chunks' histograms.
 // Measured (MI355X, logits N(0, 2.5^2)): see the table in the launch function.
 #include <algorithm>
+#include <type_traits>
 
 #include "nb_mx.hpp"
 
 namespace nb {
 
 constexpr int64_t kTokenMaxV = 1 << 20;
-constexpr int kTokenLocalV = 16384;                  // rows that one workgroup handles from beginning to end
+constexpr int kTokenLocalV = 16376;                  // rows that one workgroup handles from beginning to end
 constexpr int kGroup = 8;                            // entries of a lane's load: aligned pieces of memory, whatever the row's start
 constexpr int kSegGroups = 64;                       // a segment: the groups of one load of a wave
 constexpr int kTokenMaxSegs = kTokenMaxV / (kGroup * kSegGroups) + 1;
@@ -25,7 +26,7 @@ constexpr int kTokenMaxChunks = kTokenMaxV / (kGroup * kChunkGroups) + 1;
 constexpr int kSlots = 256;                          // bins of 1/8 of an octave of the weights below the maximum; the last
                                                      // one holds all that is further below
 constexpr int kSlotsPerOctave = 8;
-constexpr int kTokenList = 4096;                     // entries of a border bin that fit LDS
+constexpr uint32_t kTokenList = 4096;                     // entries of a border bin that fit LDS
 
 // Order-preserving keys; 0: an entry that is never drawn (NaN, -inf; no int32 entry is).  -0 and +0 are one key.
 __device__ __forceinline__ uint32_t token_key(float v)
@@ -48,6 +49,23 @@ struct TokenKey {
         mx_load8(v, p);
 #pragma unroll
         for (int e = 0; e < 8; e++) k[e] = token_key(v[e]);
+    }
+    static __device__ __forceinline__ void value8(double (&d)[8], const T *p)
+    {
+        float v[8];
+        mx_load8(v, p);
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] = (double)fmaxf(v[e], -__builtin_inff());       // NaN: -inf
+    }
+    static __device__ __forceinline__ uint32_t key_of(double v) { return token_key((float)v); }
+    // logits as they compare cheapest; plain(k): the logit of a key, for windows of them (0 and what is above +inf's key: the
+    // ends of what can be drawn)
+    typedef float Plain;
+    static __device__ __forceinline__ void plain8(float (&v)[8], const T *p) { mx_load8(v, p); }
+    static __device__ __forceinline__ float plain(uint32_t k)
+    {
+        return k < 0x00800000u ? -3.402823466e38f : k > 0xFF800000u ? __builtin_inff()
+                                                                    : __builtin_bit_cast(float, k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu));
     }
     // a key not above (not below) those of all logits of at least (at most) v, a few units of fp32 off
     static __device__ __forceinline__ uint32_t below(double v)
@@ -74,6 +92,19 @@ struct TokenKey<int32_t> {
 #pragma unroll
         for (int e = 0; e < 8; e++) k[e] ^= 0x80000000u;
     }
+    static __device__ __forceinline__ void value8(double (&d)[8], const int32_t *p)
+    {
+        const int4 a = reinterpret_cast<const int4 *>(p)[0], b = reinterpret_cast<const int4 *>(p)[1];
+        d[0] = a.x, d[1] = a.y, d[2] = a.z, d[3] = a.w, d[4] = b.x, d[5] = b.y, d[6] = b.z, d[7] = b.w;
+    }
+    static __device__ __forceinline__ uint32_t key_of(double v) { return (uint32_t)(int32_t)v ^ 0x80000000u; }
+    typedef int32_t Plain;
+    static __device__ __forceinline__ void plain8(int32_t (&v)[8], const int32_t *p)
+    {
+        const int4 a = reinterpret_cast<const int4 *>(p)[0], b = reinterpret_cast<const int4 *>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    static __device__ __forceinline__ int32_t plain(uint32_t k) { return (int32_t)(k ^ 0x80000000u); }
     static __device__ __forceinline__ uint32_t below(double v)
     {
         if (!(v > -2147483640.0)) return 0u;
@@ -98,15 +129,37 @@ struct TokenArgs {
     uint8_t *workspace;
 };
 
-// A row as groups of eight entries that start at multiples of 16 bytes: group j holds the entries 8 j - lead ...
+// A row as groups of eight entries that start at multiples of 16 bytes: group j holds the entries 8 j - lead ...  The
+// first and the last group may reach past the row's ends: their keys are put into LDS once, entry by entry.
+struct TokenEdges {
+    uint32_t key[2][kGroup], have[2];
+};
 template <typename T>
 struct TokenLogits {
     const T *row;
     int V, lead, groups;
-    __device__ __forceinline__ TokenLogits(const void *logits, int64_t r, int V_) : row((const T *)logits + r * V_), V(V_)
+    const TokenEdges *edges;
+    __device__ __forceinline__ TokenLogits(const void *logits, int64_t r, int V_, const TokenEdges *e = nullptr)
+        : row((const T *)logits + r * V_), V(V_), edges(e)
     {
         lead = (int)(((uintptr_t)row & 15) / sizeof(T));
         groups = (V + lead + kGroup - 1) / kGroup;
+    }
+    // by the first wave; the edges are there behind the caller's next barrier
+    __device__ __forceinline__ void find_edges(TokenEdges *e) const
+    {
+        if (threadIdx.x >= 64) return;
+        const int lane = threadIdx.x, i = (lane < 8 ? 0 : groups - 1) * kGroup - lead + (lane & 7);
+        const bool in = lane < 16 && i >= 0 && i < V;    // lanes 0-7: the first group, 8-15: the last
+        const uint32_t k = in ? TokenKey<T>::key1(row + i) : 0u;
+        const uint64_t have = __ballot(in && TokenKey<T>::drawable(k));
+        if (lane < 16) e->key[lane >> 3][lane & 7] = k;
+        if (lane == 0) e->have[0] = (uint32_t)have & 255u, e->have[1] = (uint32_t)(have >> 8) & 255u;
+    }
+    __device__ __forceinline__ bool whole(int j) const
+    {
+        const int i0 = j * kGroup - lead;
+        return i0 >= 0 && i0 + kGroup <= V;
     }
     // keys of group j and which of its entries can be drawn
     __device__ __forceinline__ uint32_t load(uint32_t (&k)[8], int j) const
@@ -118,49 +171,76 @@ struct TokenLogits {
 #pragma unroll
             for (int e = 0; e < 8; e++) have |= (uint32_t)TokenKey<T>::drawable(k[e]) << e;
         } else {
+            const int which = j ? 1 : 0;
+            have = edges->have[which];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool in = i0 + e >= 0 && i0 + e < V;
-                k[e] = in ? TokenKey<T>::key1(row + i0 + e) : 0u;
-                have |= (uint32_t)(in && TokenKey<T>::drawable(k[e])) << e;
-            }
+            for (int e = 0; e < 8; e++) k[e] = edges->key[which][e];
         }
         return have;
     }
+    // an edge group's logits, -inf for those that are not there or cannot be drawn
+    static __device__ __forceinline__ void edge_values(double (&d)[8], int j, const TokenEdges *edges)
+    {
+        const int which = j ? 1 : 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            d[e] = edges->have[which] >> e & 1 ? TokenKey<T>::value(edges->key[which][e]) : -__builtin_inf();
+    }
 };
 
-// 2^t for t <= 0 as an integer multiple of 2^-frac, rounded: 2^t = 2^n 2^f with n the nearest integer, 2^f by its Taylor
-// sum in f ln 2, |f ln 2| <= 0.347, to the 12th power (the rest is below 2e-16 of it), then a shift of the 53-bit
-// significand.
-__device__ __forceinline__ uint64_t token_exp2(double t, int frac)
+// 2^(u / 256) for u <= 0 as an integer multiple of 2^-frac, rounded (frac <= 51).  u = 256 n + j + r with |r| <= 1/2 and
+// 0 <= j < 256: 2^n by the exponent, 2^(j / 256) from a table, 2^(r / 256) by its Taylor sum to the fourth power, whose rest
+// is below 4e-17.  Adding 1.5 * 2^52 rounds u to an integer that then is the low word; adding 2^52 does the same for the
+// weight, whose bits below the exponent are the integer.  Fourteen 64-bit operations; the exponentials bound the long rows.
+constexpr int kExpTable = 256;
+struct TokenExp {
+    double power[kExpTable];                             // 2^(j / 256), j = 0 ... 255
+};
+constexpr TokenExp token_powers()
 {
-    if (!(t > -64.0)) return 0;
-    constexpr double ln2 = 0.69314718055994530942;
-    const double n = rint(t), f = (t - n) * ln2;
-    constexpr double c[13] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
-                              1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
-    double p = c[12];
-#pragma unroll
-    for (int i = 11; i >= 0; i--) p = fma(p, f, c[i]);
-    const uint64_t bits = __builtin_bit_cast(uint64_t, p);
-    const int shift = 1075 - frac - (int)(bits >> 52) - (int)n;      // p = significand * 2^(exponent - 1075)
-    if (shift >= 64) return 0;
-    const uint64_t m = (bits & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull;
-    return shift ? (m + (1ull << (shift - 1))) >> shift : m;
+    TokenExp t{};
+    for (int j = 0; j < kExpTable; j++) {
+        const double x = 0.69314718055994530942 * j / kExpTable;
+        double sum = 0.0, term = 1.0;
+        for (int i = 1; i < 32; i++) sum += term, term = term * x / i;
+        t.power[j] = sum;
+    }
+    return t;
+}
+__device__ const TokenExp kTokenPowers = token_powers();
+// the table into LDS, by the whole workgroup; the caller's next barrier makes it visible
+__device__ __forceinline__ void token_exp_table(TokenExp *t)
+{
+    for (int j = threadIdx.x; j < kExpTable; j += blockDim.x) t->power[j] = kTokenPowers.power[j];
+}
+__device__ __forceinline__ uint64_t token_exp2(double u, int frac, const TokenExp *t)
+{
+    constexpr double a = 0.69314718055994530942 / kExpTable;
+    constexpr double c2 = a * a / 2, c3 = a * a * a / 6, c4 = a * a * a * a / 24;
+    constexpr double half = 6755399441055744.0;          // 1.5 * 2^52
+    u = fmax(u, -20000.0);                               // 2^-78: 0 for every frac
+    const double y = u + half;
+    const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, y);
+    const double r = u - (y - half);
+    const double p = fma(fma(fma(fma(c4, r, c3), r, c2), r, a), r, 1.0) * t->power[i & (kExpTable - 1)];
+    const double v = __builtin_amdgcn_ldexp(p, (i >> 8) + frac) + 4503599627370496.0;
+    return __builtin_bit_cast(uint64_t, v) & 0xFFFFFFFFFFFFFull;
 }
 
 // How a row's logits become weights, relative to a maximum (the row's, or a chunk's)
 template <typename T>
 struct TokenScale {
     uint32_t kmax;
-    double vmax, rate;      // octaves of the weight per unit of the logits
+    double vmax, rate256;   // 256 times the octaves of the weight per unit of the logits
+    double per;             // bins per unit
     int frac;
-    __device__ __forceinline__ TokenScale(uint32_t kmax_, double rate_, int frac_)
-        : kmax(kmax_), vmax(TokenKey<T>::value(kmax_)), rate(rate_), frac(frac_) {}
+    const TokenExp *table;
+    __device__ __forceinline__ TokenScale(uint32_t kmax_, double rate, int frac_, const TokenExp *t)
+        : kmax(kmax_), vmax(TokenKey<T>::value(kmax_)), rate256(rate * kExpTable), per(rate * kSlotsPerOctave), frac(frac_), table(t) {}
     __device__ __forceinline__ uint64_t weight(uint32_t k) const
     {
-        if (k == kmax) return 1ull << frac;                          // also where both are +inf
-        return token_exp2((TokenKey<T>::value(k) - vmax) * rate, frac);
+        const uint64_t w = token_exp2((TokenKey<T>::value(k) - vmax) * rate256, frac, table);
+        return k == kmax ? 1ull << frac : w;             // also where both are +inf
     }
     // Bins lie on one grid for all chunks of a row; they are the same for equal logits and rise with them.
     static __device__ __forceinline__ double bin(uint32_t k, double rate)
@@ -171,7 +251,7 @@ struct TokenScale {
     __device__ __forceinline__ int slot(uint32_t k, double top) const
     {
         if (k == kmax) return 0;
-        const double d = top - bin(k, rate);
+        const double d = top - floor(TokenKey<T>::value(k) * per);
         return d < kSlots - 1 ? (int)d : kSlots - 1;
     }
 };
@@ -190,7 +270,9 @@ struct TokenSettings {
         top_p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
         min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
     }
-    __device__ __forceinline__ bool cut() const { return top_k > 0 || top_p < 1.0; }
+    // whether anything is cut off a row, and whether by a count or a sum
+    __device__ __forceinline__ bool cut() const { return top_k > 0 || top_p < 1.0 || min_p > 0.0; }
+    __device__ __forceinline__ bool ranked() const { return top_k > 0 || top_p < 1.0; }
 };
 
 template <typename U>
@@ -231,6 +313,9 @@ __device__ __forceinline__ uint64_t token_bar(uint32_t word, uint64_t all)
 template <typename T>
 __global__ __launch_bounds__(256) void sample_short_kernel(TokenArgs a)
 {
+    __shared__ TokenExp table;
+    token_exp_table(&table);
+    __syncthreads();
     const int lane = threadIdx.x & 63, V = a.V;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= a.R) return;                              // whole waves; no barrier follows
@@ -248,10 +333,10 @@ __global__ __launch_bounds__(256) void sample_short_kernel(TokenArgs a)
         if (lane == 0) a.out[row] = __builtin_ctzll(at);
         return;
     }
-    const TokenScale<T> scale(kmax, set.rate, a.frac_bits);
+    const TokenScale<T> scale(kmax, set.rate, a.frac_bits, &table);
     uint64_t w = have ? scale.weight(key) : 0;
     bool keep = have;
-    if (set.cut()) {
+    if (set.ranked()) {
         int rank = 0;                                    // entries before this one, and their weight
         uint64_t before = 0;
         for (int j = 0; j < V; j++) {
@@ -284,107 +369,214 @@ struct TokenChunk {
 };
 static_assert(sizeof(TokenChunk) % 16 == 0, "records of the workspace");
 
+// A workgroup takes chunk after chunk, the next one's loads under way while it works on one (a workgroup per chunk spent
+// most of its life waiting for them: 46 us instead of 33 for the exponentials of 256 x 131072).
+constexpr int kChunkGrid = 512;
 template <typename T>
 __global__ __launch_bounds__(512) void token_chunk_kernel(TokenArgs a)
 {
+    constexpr int WORDS = sizeof(T) / 2;                 // 16-byte words of a group
+    __shared__ TokenExp table;
+    __shared__ TokenEdges edges;
     __shared__ uint64_t hist_w[kSlots], sh_sum;
-    __shared__ uint32_t hist_c[kSlots], sh_max[8], sh_have[8];
+    __shared__ uint32_t hist_c[kSlots];
+    __shared__ double sh_max[2][8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x / a.chunks;
-    const int chunk = (int)(blockIdx.x - row * a.chunks);
-    const TokenSettings set(a, row);
-    const TokenLogits<T> x(a.logits, row, a.V);
-    TokenChunk *out = reinterpret_cast<TokenChunk *>(a.workspace) + blockIdx.x;
-    uint32_t k[2][8], have[2], m = 0;
+    const uint32_t items = (uint32_t)(a.R * a.chunks);
+    uint4 next[2][WORDS];
+    bool next_whole[2] = {false, false};
+    const auto request = [&](uint32_t item) {
+        if (item >= items) return;
+        const uint32_t row = item / (uint32_t)a.chunks;
+        const TokenLogits<T> x(a.logits, row, a.V);
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-        const int j = chunk * kChunkGroups + q * 512 + tid;
-        have[q] = 0;
-        if (j < x.groups) have[q] = x.load(k[q], j);
-    }
+        for (int q = 0; q < 2; q++) {
+            const int j = (int)(item - row * a.chunks) * kChunkGroups + q * 512 + tid;
+            next_whole[q] = x.whole(j);
+            if (next_whole[q]) {
 #pragma unroll
-    for (int q = 0; q < 2; q++)
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (have[q] >> e & 1) m = k[q][e] > m ? k[q][e] : m;
-    const uint64_t any = __ballot(have[0] | have[1]);
-    m = wave_max(m);
-    if (lane == 0) sh_max[wave] = m, sh_have[wave] = any != 0;
+                for (int w = 0; w < WORDS; w++) next[q][w] = reinterpret_cast<const uint4 *>(x.row + (j * kGroup - x.lead))[w];
+            }
+        }
+    };
+    request(blockIdx.x);
     for (int t = tid; t < kSlots; t += 512) hist_w[t] = 0, hist_c[t] = 0;
+    token_exp_table(&table);
     if (tid == 0) sh_sum = 0;
-    __syncthreads();
-    uint32_t h = 0;
+    int turn = 0;
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x, turn ^= 1) {
+        const int64_t row = item / (uint32_t)a.chunks;
+        const int chunk = (int)(item - (uint32_t)row * a.chunks);
+        const TokenLogits<T> x(a.logits, row, a.V);
+        const TokenSettings set(a, row);
+        TokenChunk *out = reinterpret_cast<TokenChunk *>(a.workspace) + item;
+        double d[2][8];
+        bool whole[2];
 #pragma unroll
-    for (int w = 0; w < 8; w++) m = sh_max[w] > m ? sh_max[w] : m, h |= sh_have[w];
-    if (h && !set.greedy) {
-        const TokenScale<T> scale(m, set.rate, a.frac_bits);
-        const double top = TokenScale<T>::bin(m, set.rate);
-        const bool cut = set.cut(), counted = set.top_k > 0;
-        uint64_t sum = 0;
+        for (int q = 0; q < 2; q++) {
+            whole[q] = next_whole[q];
+            TokenKey<T>::value8(d[q], reinterpret_cast<const T *>(next[q]));
+        }
+        request(item + gridDim.x);
+        const int j0 = chunk * kChunkGroups + tid;
+        if (chunk == 0 || chunk * kChunkGroups + kChunkGroups >= x.groups) {     // chunks with an edge of the row
+            __syncthreads();
+            x.find_edges(&edges);
+            __syncthreads();
+        }
 #pragma unroll
         for (int q = 0; q < 2; q++)
+            if (!whole[q]) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (have[q] >> e & 1) {
-                    const uint64_t w = scale.weight(k[q][e]);
-                    sum += w;
-                    if (cut) {
-                        const int s = scale.slot(k[q][e], top);
-                        atomicAdd((unsigned long long *)&hist_w[s], (unsigned long long)w);
-                        if (counted) atomicAdd(&hist_c[s], 1u);
+                for (int e = 0; e < 8; e++) d[q][e] = -__builtin_inf();
+                if (j0 + q * 512 < x.groups) x.edge_values(d[q], j0 + q * 512, &edges);
+            }
+        double m = -__builtin_inf();
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = fmax(m, fmax(d[0][e], d[1][e]));
+        m = wave_max(m);
+        if (lane == 0) sh_max[turn][wave] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; w++) m = fmax(m, sh_max[turn][w]);
+        const bool any = m > -__builtin_inf();
+        if (any && !set.greedy) {
+            if (m == __builtin_inf()) {                  // the infinities share the weight; all others have none
+#pragma unroll
+                for (int q = 0; q < 2; q++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) d[q][e] = d[q][e] == m ? 0.0 : -__builtin_inf();
+            }
+            const double from = m == __builtin_inf() ? 0.0 : m, rate256 = set.rate * kExpTable;
+            const double per = set.rate * kSlotsPerOctave, top = floor(from * per);
+            const bool cut = set.cut(), counted = set.top_k > 0;
+            uint64_t sum = 0;
+            // eight at a time: their chains of dependent operations run side by side
+            const auto take = [&](const double (&v)[8]) {
+                uint64_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = token_exp2((v[e] - from) * rate256, a.frac_bits, &table);
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum += w[e];
+                if (cut) {
+                    int at[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) at[e] = (int)fmin(top - floor(v[e] * per), (double)(kSlots - 1));
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (w[e]) atomicAdd((unsigned long long *)&hist_w[at[e]], (unsigned long long)w[e]);
+                    if (counted) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (v[e] > -__builtin_inf()) atomicAdd(&hist_c[at[e]], 1u);
                     }
                 }
-        sum = wave_sum(sum);
-        if (lane == 0) atomicAdd((unsigned long long *)&sh_sum, (unsigned long long)sum);
-        __syncthreads();
-        if (cut)
-            for (int t = tid; t < kSlots; t += 512) out->weight[t] = hist_w[t], out->count[t] = hist_c[t];
+            };
+            take(d[0]);
+            take(d[1]);
+            sum = wave_sum(sum);
+            if (lane == 0) atomicAdd((unsigned long long *)&sh_sum, (unsigned long long)sum);
+            __syncthreads();
+            if (cut)
+                for (int t = tid; t < kSlots; t += 512) {
+                    out->weight[t] = hist_w[t], out->count[t] = hist_c[t];
+                    hist_w[t] = 0, hist_c[t] = 0;        // for the next chunk, behind its first barrier
+                }
+        }
+        if (tid == 0) {
+            out->sum = sh_sum, out->kmax = any ? TokenKey<T>::key_of(m) : 0u, out->have = any;
+            sh_sum = 0;
+        }
     }
-    if (tid == 0) out->sum = sh_sum, out->kmax = m, out->have = h;
 }
 
 // ---- a workgroup per row ----------------------------------------------------------------------------------------------
-// LOCAL: from the logits alone; else from the chunks' records.
-template <typename T, int THREADS, bool LOCAL>
+// HELD > 0: rows of at most HELD groups per thread, kept in registers; HELD = 0: longer ones, from the chunks' records, read
+// again where entries matter.  The passes over the row are few and their code is kept short:
+// with every step inlined where it is used (145 KB) fetching instructions took longer than all else.
+struct TokenEntry {
+    uint32_t key;
+    int index;
+};
+
+template <typename T, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
 {
+    constexpr bool LOCAL = HELD > 0;
     constexpr int WAVES = THREADS / 64;
     constexpr int SEGS = LOCAL ? kTokenLocalV / (kGroup * kSegGroups) + 1 : kTokenMaxSegs;
-    __shared__ uint64_t seg_w[SEGS];
-    __shared__ uint32_t seg_c[SEGS];
+    constexpr int CHUNKS = LOCAL ? 1 : kTokenMaxChunks;
+    constexpr uint32_t kList = LOCAL ? 1024 : kTokenList;
+    __shared__ TokenExp table;
+    __shared__ TokenEdges edges;
+    __shared__ uint64_t seg_w[SEGS];                     // what is kept of a segment; tie counts before
     __shared__ double slot_w[kSlots];
-    __shared__ uint64_t hist_w[kSlots];                  // LOCAL: by slot; in select(): by digit
+    __shared__ uint64_t hist_w[kSlots];                  // LOCAL: by slot; later by digit
     __shared__ uint32_t hist_c[kSlots], slot_c[kSlots];
-    __shared__ uint32_t list[kTokenList];
-    __shared__ double chunk_f[LOCAL ? 1 : kTokenMaxChunks];
-    __shared__ int chunk_off[LOCAL ? 1 : kTokenMaxChunks];
-    __shared__ uint32_t sh_key[WAVES], sh_have[WAVES], sh_n, sh_count, sh_ties;
+    __shared__ TokenEntry list[kList];                   // the entries of the border's slot
+    __shared__ double chunk_f[CHUNKS];
+    __shared__ int chunk_off[CHUNKS];
+    __shared__ uint64_t chunk_w[CHUNKS];                 // what is kept of a chunk
+    __shared__ uint32_t sh_key[WAVES], sh_have[WAVES], low_c[WAVES], sh_n, sh_count, sh_ties;
     __shared__ uint64_t sh_sum;
-    __shared__ double sh_before;
+    __shared__ double low_w[WAVES], sh_before;
     __shared__ int sh_at;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
+    token_exp_table(&table);
+    if (tid == 0) sh_at = a.V;
+    if (LOCAL)
+        for (int t = tid; t < kSlots; t += THREADS) hist_w[t] = 0, hist_c[t] = 0;
+    const TokenLogits<T> x(a.logits, row, a.V, &edges);
+    x.find_edges(&edges);
+    __syncthreads();
     const TokenSettings set(a, row);
-    const TokenLogits<T> x(a.logits, row, a.V);
     const int segs = (x.groups + kSegGroups - 1) / kSegGroups;
     const TokenChunk *chunk = reinterpret_cast<const TokenChunk *>(a.workspace) + row * a.chunks;
-    // f(keys, which can be drawn, first entry's index, segment): every wave takes whole segments
-    const auto for_groups = [&](auto &&f) {
-        for (int s = wave; s < segs; s += WAVES) {
-            uint32_t k[8], have = 0;
-            const int j = s * kSegGroups + lane;
-            if (j < x.groups) have = x.load(k, j);
-            f(k, have, j * kGroup - x.lead, s);
+    uint32_t held[LOCAL ? HELD : 1][8], held_have[LOCAL ? HELD : 1];
+    if constexpr (LOCAL) {
+#pragma unroll
+        for (int q = 0; q < HELD; q++) {
+            const int j = q * THREADS + tid;
+            held_have[q] = 0;
+            if (j < x.groups) held_have[q] = x.load(held[q], j);
+#pragma unroll
+            for (int e = 0; e < 8; e++) held[q][e] = held_have[q] >> e & 1 ? held[q][e] : 0u;
+        }
+    }
+    // f(keys, which of them there are, the first one's index, segment) for the segments seg0 ... seg1 - 1: every wave takes
+    // whole segments; from memory, AHEAD of them are under way at once
+    const auto for_groups = [&](auto ahead, int seg0, int seg1, auto &&f) {
+        if constexpr (LOCAL) {
+#pragma unroll
+            for (int q = 0; q < HELD; q++)
+                if (q * WAVES + wave < segs) f(held[q], held_have[q], (q * THREADS + tid) * kGroup - x.lead, q * WAVES + wave);
+        } else {
+            constexpr int AHEAD = decltype(ahead)::value;
+#pragma unroll 1
+            for (int s = seg0 + wave; s < seg1; s += AHEAD * WAVES) {
+                uint32_t k[AHEAD][8], have[AHEAD];
+#pragma unroll
+                for (int q = 0; q < AHEAD; q++) {
+                    const int j = (s + q * WAVES) * kSegGroups + lane;
+                    have[q] = 0;
+                    if (s + q * WAVES < seg1 && j < x.groups) have[q] = x.load(k[q], j);
+                }
+#pragma unroll
+                for (int q = 0; q < AHEAD; q++)
+                    if (s + q * WAVES < seg1)
+                        f(k[q], have[q], ((s + q * WAVES) * kSegGroups + lane) * kGroup - x.lead, s + q * WAVES);
+            }
         }
     };
+    const std::integral_constant<int, 1> one_ahead{};
     // the row's maximum
     uint32_t m = 0, any = 0;
     if (LOCAL) {
-        for_groups([&](const uint32_t (&k)[8], uint32_t have, int, int) {
+        for_groups(one_ahead, 0, segs, [&](const uint32_t (&k)[8], uint32_t have, int, int) {
             any |= have;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (have >> e & 1) m = k[e] > m ? k[e] : m;
+            for (int e = 0; e < 8; e++) m = k[e] > m ? k[e] : m;
         });
     } else {
         for (int c = tid; c < a.chunks; c += THREADS)
@@ -393,7 +585,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     m = wave_max(m);
     any = __ballot(any) != 0;
     if (lane == 0) sh_key[wave] = m, sh_have[wave] = any;
-    if (tid == 0) sh_at = a.V;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WAVES; w++) m = sh_key[w] > m ? sh_key[w] : m, any |= sh_have[w];
@@ -401,149 +592,124 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
         if (tid == 0) a.out[row] = -1;
         return;
     }
-    const TokenScale<T> scale(m, set.rate, a.frac_bits);
-    const double top = TokenScale<T>::bin(m, set.rate);
-    const double one = (double)(1ull << a.frac_bits);
     if (set.greedy) {
-        for_groups([&](const uint32_t (&k)[8], uint32_t have, int i0, int) {
-            for (int e = 0; e < 8; e++)
-                if ((have >> e & 1) && k[e] == m) {
-                    atomicMin(&sh_at, i0 + e);
-                    break;
-                }
+        int seg0 = 0, seg1 = segs;
+        if constexpr (!LOCAL) {                          // the first chunk with that maximum
+            for (int c = tid; c < a.chunks; c += THREADS)
+                if (chunk[c].have && chunk[c].kmax == m) atomicMin(&sh_at, c);
+            __syncthreads();
+            seg0 = sh_at * (kChunkGroups / kSegGroups);
+            seg1 = seg0 + kChunkGroups / kSegGroups < segs ? seg0 + kChunkGroups / kSegGroups : segs;
+            __syncthreads();
+            if (tid == 0) sh_at = a.V;
+            __syncthreads();
+        }
+        for_groups(one_ahead, seg0, seg1, [&](const uint32_t (&k)[8], uint32_t have, int i0, int) {
+            int first = a.V;
+#pragma unroll
+            for (int e = 7; e >= 0; e--) first = (have >> e & 1) && k[e] == m ? i0 + e : first;
+            if (first < a.V) atomicMin(&sh_at, first);
         });
         __syncthreads();
         if (tid == 0) a.out[row] = sh_at;
         return;
     }
-
+    const TokenScale<T> scale(m, set.rate, a.frac_bits, &table);
+    const double top = TokenScale<T>::bin(m, set.rate);
+    // The smallest key that reaches min_p (weights rise with keys): 64 keys at a time, six bits of it per turn.
+    uint32_t min_key = 0;
+    if (set.min_p > 0.0) {
+        const double min_w = std::min(set.min_p, 1.0) * (double)(1ull << a.frac_bits);
+#pragma unroll 1
+        for (int shift = 26;; shift = shift > 2 ? shift - 6 : 0) {
+            const uint64_t k = (uint64_t)min_key + ((uint64_t)lane << shift);    // none below min_key reaches it
+            const uint64_t hit = __ballot(k >= m || (double)scale.weight((uint32_t)k) >= min_w);
+            if (hit & 1) break;
+            min_key += ((hit ? (uint32_t)__builtin_ctzll(hit) : 64u) - 1) << shift;
+            min_key += 1;
+        }
+    }
     if constexpr (!LOCAL) {
         for (int c = tid; c < a.chunks; c += THREADS) {
             const uint32_t cm = chunk[c].kmax;
             const double d = cm == m ? 0.0 : top - TokenScale<T>::bin(cm, set.rate);
             chunk_off[c] = !chunk[c].have ? kSlots : d < kSlots - 1 ? (int)d : kSlots - 1;
             chunk_f[c] = !chunk[c].have ? 0.0 : cm == m ? 1.0 : exp2((TokenKey<T>::value(cm) - scale.vmax) * set.rate);
+            chunk_w[c] = !chunk[c].have ? 0 : chunk[c].sum;
         }
         __syncthreads();
     }
     // what is kept: keys above `key`, and `ties` of those equal to it, the first ones
     uint32_t key = 0, ties = 0xFFFFFFFFu, equal = 0;
-    if (set.cut()) {
+    int border = kSlots;                                 // the slot it lies in; kSlots: all are kept
+    bool listed = false;                                 // whether `list` holds all of that slot,
+    uint32_t list_n = 0;                                 // and how many it has
+    if (set.ranked() || (!LOCAL && set.cut())) {
         // ---- the row's histogram -------------------------------------------------------------------------------------
         if (LOCAL) {
-            for (int t = tid; t < kSlots; t += THREADS) hist_w[t] = 0, hist_c[t] = 0;
-            __syncthreads();
-            for_groups([&](const uint32_t (&k)[8], uint32_t have, int, int) {
-                for (int e = 0; e < 8; e++)
-                    if (have >> e & 1) {
-                        const int s = scale.slot(k[e], top);
-                        atomicAdd((unsigned long long *)&hist_w[s], (unsigned long long)scale.weight(k[e]));
-                        if (set.top_k) atomicAdd(&hist_c[s], 1u);
-                    }
+            for_groups(one_ahead, 0, segs, [&](const uint32_t (&k)[8], uint32_t have, int, int) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint64_t w = scale.weight(k[e]);
+                    const int s = scale.slot(k[e], top);
+                    if ((have >> e & 1) && w) atomicAdd((unsigned long long *)&hist_w[s], (unsigned long long)w);
+                    if ((have >> e & 1) && set.top_k) atomicAdd(&hist_c[s], 1u);
+                }
             });
             __syncthreads();
             for (int t = tid; t < kSlots; t += THREADS) slot_w[t] = (double)hist_w[t], slot_c[t] = hist_c[t];
         } else {
             // a chunk's bin s lies chunk_off bins lower in the row, its weights are chunk_f of the row's; chunk after chunk, so
-            // the sums have one order.  The last slot also takes all that lies below it (a wave of its own).
+            // the sums have one order.  The last slot also takes all that lies below it (the other waves).
             if (tid < kSlots - 1) {
                 double w = 0.0;
                 uint32_t n = 0;
 #pragma unroll 8
                 for (int c = 0; c < a.chunks; c++) {
-                    const int s = tid - chunk_off[c];
-                    if (s >= 0) w += chunk_f[c] * (double)chunk[c].weight[s], n += chunk[c].count[s];
+                    const int s = tid - chunk_off[c], at = s > 0 ? s : 0;        // no branch: the loads go out together
+                    const double f = s >= 0 ? chunk_f[c] : 0.0;
+                    w += f * (double)chunk[c].weight[at], n += s >= 0 ? chunk[c].count[at] : 0;
                 }
                 slot_w[tid] = w, slot_c[tid] = n;
-            } else if (wave == kSlots / 64) {
+            } else if (wave >= kSlots / 64) {
+                constexpr int kWaves = WAVES - kSlots / 64 > 0 ? WAVES - kSlots / 64 : 1;
                 double w = 0.0;
                 uint32_t n = 0;
-                for (int c = 0; c < a.chunks; c++) {
-                    if (chunk_off[c] >= kSlots) continue;
-                    for (int s = kSlots - 1 - chunk_off[c] + lane; s < kSlots; s += 64)
-                        w += chunk_f[c] * (double)chunk[c].weight[s], n += chunk[c].count[s];
+                for (int c = wave - kSlots / 64; c < a.chunks; c += kWaves) {
+#pragma unroll
+                    for (int q = 0; q < kSlots / 64; q++) {
+                        const int s = q * 64 + lane;
+                        if (s + chunk_off[c] >= kSlots - 1 && chunk_off[c] < kSlots)
+                            w += chunk_f[c] * (double)chunk[c].weight[s], n += chunk[c].count[s];
+                    }
                 }
                 w = wave_sum(w), n = wave_sum(n);
-                if (lane == 0) slot_w[kSlots - 1] = w, slot_c[kSlots - 1] = n;
+                if (lane == 0) low_w[wave] = w, low_c[wave] = n;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                double w = 0.0;
+                uint32_t n = 0;
+                for (int v = kSlots / 64; v < WAVES; v++) w += low_w[v], n += low_c[v];
+                slot_w[kSlots - 1] = w, slot_c[kSlots - 1] = n;
             }
         }
         __syncthreads();
-        // ---- borders ---------------------------------------------------------------------------------------------------
+        // ---- the borders, one after the other: top_k, top_p, min_p -----------------------------------------------------
         double total = 0.0;                              // what top_p is a part of
         bool have_total = false;
-        // Digit by digit among the entries that `each` hands out and f accepts: the shortest prefix of at least k
-        // entries, or of a weight of at least target, `before` entries or weight lying above all of them.  The row has to
-        // reach it among them.
-        const auto digits = [&](auto &&each, bool by_count, int64_t k, double target, uint32_t before_c, double before_w) {
-            uint32_t prefix = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                __syncthreads();
-                for (int t = tid; t < kSlots; t += THREADS) hist_w[t] = 0, hist_c[t] = 0;
-                __syncthreads();
-                each([&](uint32_t q) {
-                    if (shift == 24 || q >> (shift + 8) == prefix) {
-                        atomicAdd(&hist_c[(q >> shift) & 255], 1u);
-                        atomicAdd((unsigned long long *)&hist_w[(q >> shift) & 255], (unsigned long long)scale.weight(q));
-                    }
-                });
-                __syncthreads();
-                if (wave == 0) {                         // lane l: the digits 255 - 4 l down to 252 - 4 l
-                    uint32_t c[4], cs = 0;
-                    uint64_t w[4], ws = 0;
+#pragma unroll 1
+        for (int which = 0; which < 3; which++) {
+            const bool by_count = which == 0;
+            if (which == 0 ? !set.top_k : which == 1 ? !(set.top_p < 1.0) : LOCAL || !(set.min_p > 0.0)) continue;
+            if (which == 1 && !have_total) {
+                double w = 0.0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        c[e] = hist_c[255 - 4 * lane - e], w[e] = hist_w[255 - 4 * lane - e];
-                        cs += c[e], ws += w[e];
-                    }
-                    uint32_t ca = wave_scan(cs, lane) - cs;
-                    uint64_t wa = wave_scan(ws, lane) - ws;
-                    int found = -1;
-                    uint32_t fc = 0, fn = 0;
-                    uint64_t fw = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const bool here = c[e] && (by_count ? (int64_t)before_c + ca + c[e] >= k
-                                                            : before_w + (double)(wa + w[e]) >= target);
-                        if (found < 0 && here) found = 255 - 4 * lane - e, fc = ca, fw = wa, fn = c[e];
-                        ca += c[e], wa += w[e];
-                    }
-                    // the last digit that holds anything, should rounding put the target above all
-                    const uint64_t hit = __ballot(found >= 0), some = __ballot(cs != 0);
-                    if (hit) {
-                        if (lane == __builtin_ctzll(hit)) sh_at = found, sh_count = fc, sh_sum = fw, sh_ties = fn;
-                    } else if (some && lane == 63 - __builtin_clzll(some)) {
-                        uint32_t cb = ca - cs;
-                        uint64_t wb = wa - ws;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if (c[e]) sh_at = 255 - 4 * lane - e, sh_ties = c[e], sh_count = cb, sh_sum = wb;
-                            cb += c[e], wb += w[e];
-                        }
-                    }
-                }
-                __syncthreads();
-                before_c += sh_count;
-                before_w += (double)sh_sum;
-                equal = sh_ties;
-                prefix = (prefix << 8) | (uint32_t)sh_at;
+                for (int e = 0; e < 4; e++) w += slot_w[4 * lane + e];
+                total = wave_sum(w);
             }
-            key = prefix;
-            const uint64_t w = scale.weight(key);
-            if (by_count) {
-                const int64_t left = k - before_c;
-                ties = left < (int64_t)equal ? (uint32_t)left : equal;
-            } else {
-                uint32_t lo = 1, hi = equal;             // the fewest that reach the target
-                while (lo < hi) {
-                    const uint32_t mid = (lo + hi) / 2;
-                    if (before_w + (double)(mid * w) >= target) hi = mid;
-                    else lo = mid + 1;
-                }
-                ties = lo;
-            }
-            total = before_w + (double)(ties * w);
-        };
-        const auto select = [&](bool by_count, int64_t k, double target) {
+            const int64_t count = set.top_k;
+            const double target = set.top_p * total;
             __syncthreads();
             // the slot that the border lies in: lane l has the slots 4 l ... 4 l + 3
             if (wave == 0) {
@@ -558,7 +724,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                 double fw = 0.0;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const bool here = by_count ? c[e] && (int64_t)ca + c[e] >= k : w[e] > 0.0 && wa + w[e] >= target;
+                    const bool here = by_count ? c[e] && (int64_t)ca + c[e] >= count : w[e] > 0.0 && wa + w[e] >= target;
                     if (found < 0 && here) found = 4 * lane + e, fc = ca, fw = wa;
                     ca += c[e], wa += w[e];
                 }
@@ -571,66 +737,248 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                 if (lane == 0) sh_n = 0;
             }
             __syncthreads();
-            const int slot = sh_at;
-            const uint32_t before_c = sh_count;
-            const double before_w = sh_before;
-            __syncthreads();
-            if (slot < 0) return;                        // the row has no more than that: nothing is cut
-            // keys that can lie in the slot, a little more than those that do
-            const double per = set.rate * kSlotsPerOctave;
-            const uint32_t lowest = slot == kSlots - 1 ? 0u : TokenKey<T>::below((top - slot) / per);
-            const uint32_t span = (slot == 0 ? 0xFFFFFFFFu : TokenKey<T>::above((top - slot + 1.0) / per)) - lowest;
-            const auto in_slot = [&](uint32_t q) { return q - lowest <= span && scale.slot(q, top) == slot; };
-            for_groups([&](const uint32_t (&q)[8], uint32_t have, int, int) {
-                for (int e = 0; e < 8; e++)
-                    if ((have >> e & 1) && in_slot(q[e])) {
+            int slot = sh_at;
+            uint32_t before_c = sh_count;
+            double before_w = sh_before;
+            if (which == 2) slot = scale.slot(min_key, top);
+            if (slot < 0 || slot > border) continue;     // the row has no more than that: nothing is cut
+            if (slot != border || !listed) {             // else the list of the border before is the one
+                // keys that can lie there, a little more than those that do
+                const uint32_t from = slot == kSlots - 1 ? 0u : TokenKey<T>::below((top - slot) / scale.per);
+                const uint32_t span = (slot == 0 ? 0xFFFFFFFFu : TokenKey<T>::above((top - slot + 1.0) / scale.per)) - from;
+                const typename TokenKey<T>::Plain lo = TokenKey<T>::plain(from), hi = TokenKey<T>::plain(from + span);
+                const auto put = [&](uint32_t k, int i) {
+                    if (scale.slot(k, top) == slot) {
                         const uint32_t at = atomicAdd(&sh_n, 1u);
-                        if (at < kTokenList) list[at] = q[e];
+                        if (at < kList) list[at] = TokenEntry{k, i};
                     }
-            });
-            __syncthreads();
-            const uint32_t n = sh_n;
-            if (n <= kTokenList) {
-                digits([&](auto &&f) { for (uint32_t i = tid; i < n; i += THREADS) f(list[i]); }, by_count, k, target,
-                       before_c, before_w);
-            } else {                                     // a slot of very many: from memory again for every digit
-                digits([&](auto &&f) {
-                    for_groups([&](const uint32_t (&q)[8], uint32_t have, int, int) {
-                        for (int e = 0; e < 8; e++)
-                            if ((have >> e & 1) && in_slot(q[e])) f(q[e]);
-                    });
-                }, by_count, k, target, before_c, before_w);
-            }
-            have_total = true;
-        };
-        if (set.top_k) select(true, set.top_k, 0.0);
-        if (set.top_p < 1.0) {
-            if (!have_total) {
-                double w = 0.0;
+                };
+                if constexpr (LOCAL) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) w += slot_w[4 * lane + e];
-                total = wave_sum(w);
+                    for (int q = 0; q < HELD; q++) {
+                        uint32_t near = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) near |= (uint32_t)(held[q][e] - from <= span) << e;
+#pragma unroll 1
+                        for (near &= held_have[q]; near; near &= near - 1) {
+                            const int e = __builtin_ctz(near);
+                            uint32_t k = held[q][0];
+#pragma unroll
+                            for (int d = 1; d < 8; d++) k = d == e ? held[q][d] : k;
+                            put(k, (q * THREADS + tid) * kGroup - x.lead + e);
+                        }
+                    }
+                } else {
+                    // one workgroup looks at the whole row: two comparisons an entry, on logits as they are
+                    constexpr int AHEAD = 4;
+                    if (tid < 2 * kGroup && (tid < kGroup ? !x.whole(0) : x.groups > 1 && !x.whole(x.groups - 1))) {
+                        const int which = tid / kGroup, e = tid % kGroup;
+                        const uint32_t k = edges.key[which][e];
+                        if ((edges.have[which] >> e & 1) && k - from <= span)
+                            put(k, (which ? x.groups - 1 : 0) * kGroup - x.lead + e);
+                    }
+#pragma unroll 1
+                    for (int s = wave; s < segs; s += AHEAD * WAVES) {
+                        typename TokenKey<T>::Plain v[AHEAD][8];
+                        bool have[AHEAD];
+#pragma unroll
+                        for (int q = 0; q < AHEAD; q++) {
+                            const int j = (s + q * WAVES) * kSegGroups + lane;
+                            have[q] = s + q * WAVES < segs && x.whole(j);
+                            if (have[q]) TokenKey<T>::plain8(v[q], x.row + (j * kGroup - x.lead));
+                        }
+#pragma unroll
+                        for (int q = 0; q < AHEAD; q++) {
+                            if (!have[q]) continue;
+                            uint32_t near = 0;
+#pragma unroll
+                            for (int e = 0; e < 8; e++) near |= v[q][e] >= lo && v[q][e] <= hi ? 1u << e : 0u;
+#pragma unroll 1
+                            for (; near; near &= near - 1) {
+                                const int i = ((s + q * WAVES) * kSegGroups + lane) * kGroup - x.lead + __builtin_ctz(near);
+                                put(TokenKey<T>::key1(x.row + i), i);    // again from memory: few of them
+                            }
+                        }
+                    }
+                }
+                __syncthreads();
+                list_n = sh_n;
+                listed = list_n <= kList;
+                border = slot;
             }
-            select(false, 0, set.top_p * total);
+            if (which == 2) continue;                    // the entries below min_key stay out by their keys
+            if (list_n <= 64) {
+                // few enough for a lane each: what lies above an entry, by comparing all pairs (every wave does the same)
+                const uint32_t q = (uint32_t)lane < list_n ? list[lane].key : 0u;
+                const uint64_t w = (uint32_t)lane < list_n ? scale.weight(q) : 0;
+                uint32_t above_c = 0, same = 0;
+                uint64_t above_w = 0;
+#pragma unroll 1
+                for (uint32_t j = 0; j < list_n; j++) {
+                    const uint32_t kj = __builtin_amdgcn_readlane(q, j);
+                    const uint64_t wj = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), j) << 32) |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, j);
+                    above_c += kj > q, above_w += kj > q ? wj : 0, same += kj == q;
+                }
+                // the border's key: the largest with which the prefix is long enough; should rounding have put the target
+                // above all of them, the smallest
+                const bool here = (uint32_t)lane < list_n && (by_count ? (int64_t)before_c + above_c + same >= count
+                                                                      : before_w + (double)(above_w + same * w) >= target);
+                const uint64_t hit = __ballot(here);
+                const uint32_t big = wave_max(here ? q : 0u), small = ~wave_max((uint32_t)lane < list_n ? ~q : 0u);
+                key = hit ? big : small;
+                const int l = __builtin_ctzll(__ballot((uint32_t)lane < list_n && q == key));
+                equal = __shfl(same, l);
+                before_c += __shfl(above_c, l);
+                before_w += (double)__shfl(above_w, l);
+            } else {
+                // Digit by digit among the slot's keys, from the list or, where it has too many, from memory every time; only
+                // the bits in which the list's keys differ (logits of 16 bits have few).
+                int top_bit = 32, low_bit = 0;
+                uint32_t prefix = 0;
+                if (listed) {
+                    uint32_t both = 0xFFFFFFFFu, one = 0;
+                    for (uint32_t i = tid; i < list_n; i += THREADS) both &= list[i].key, one |= list[i].key;
+#pragma unroll
+                    for (int o = 32; o; o >>= 1) both &= __shfl_xor(both, o), one |= __shfl_xor(one, o);
+                    if (lane == 0) sh_key[wave] = both, sh_have[wave] = one;
+                    __syncthreads();
+#pragma unroll
+                    for (int w = 0; w < WAVES; w++) both &= sh_key[w], one |= sh_have[w];
+                    const uint32_t differ = both ^ one;
+                    top_bit = differ ? 32 - __builtin_clz(differ) : 1;
+                    low_bit = differ ? __builtin_ctz(differ) : 0;
+                    prefix = top_bit < 32 ? both >> top_bit : 0;
+                }
+                // bits below low_bit are the same in all keys
+                const uint32_t rest = listed ? list[0].key & ((1u << low_bit) - 1u) : 0u;
+#pragma unroll 1
+                for (int shift = top_bit; shift > low_bit;) {
+                    const int width = shift - low_bit < 8 ? shift - low_bit : 8;
+                    shift -= width;
+                    __syncthreads();
+                    for (int t = tid; t < kSlots; t += THREADS) hist_w[t] = 0, hist_c[t] = 0;
+                    __syncthreads();
+                    const auto put = [&](uint32_t q) {
+                        if (shift + width == 32 || q >> (shift + width) == prefix) {
+                            const uint32_t d = (q >> shift) & ((1u << width) - 1u);
+                            atomicAdd(&hist_c[d], 1u);
+                            atomicAdd((unsigned long long *)&hist_w[d], (unsigned long long)scale.weight(q));
+                        }
+                    };
+                    if (listed) {
+                        for (uint32_t i = tid; i < list_n; i += THREADS) put(list[i].key);
+                    } else if constexpr (LOCAL) {
+#pragma unroll
+                        for (int q = 0; q < HELD; q++)
+#pragma unroll 1
+                            for (uint32_t left = held_have[q]; left; left &= left - 1) {
+                                uint32_t k = held[q][0];
+#pragma unroll
+                                for (int d = 1; d < 8; d++) k = d == __builtin_ctz(left) ? held[q][d] : k;
+                                if (scale.slot(k, top) == slot) put(k);
+                            }
+                    } else {
+#pragma unroll 1
+                        for (int i = tid; i < a.V; i += THREADS) {
+                            const uint32_t q = TokenKey<T>::key1(x.row + i);
+                            if (TokenKey<T>::drawable(q) && scale.slot(q, top) == slot) put(q);
+                        }
+                    }
+                    __syncthreads();
+                    if (wave == 0) {                     // lane l: the digits 255 - 4 l down to 252 - 4 l
+                        uint32_t c[4], cs = 0;
+                        uint64_t w[4], ws = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            c[e] = hist_c[255 - 4 * lane - e], w[e] = hist_w[255 - 4 * lane - e];
+                            cs += c[e], ws += w[e];
+                        }
+                        uint32_t ca = wave_scan(cs, lane) - cs;
+                        uint64_t wa = wave_scan(ws, lane) - ws;
+                        int found = -1, seen = -1;       // seen: the last digit that holds anything
+                        uint32_t fc = 0, fn = 0;
+                        uint64_t fw = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const bool here = c[e] && (by_count ? (int64_t)before_c + ca + c[e] >= count
+                                                                : before_w + (double)(wa + w[e]) >= target);
+                            if (found < 0 && (here || c[e])) {
+                                fc = ca, fw = wa, fn = c[e];
+                                seen = 255 - 4 * lane - e;
+                                if (here) found = seen;
+                            }
+                            ca += c[e], wa += w[e];
+                        }
+                        // should rounding have put the target above all of them: the last one
+                        const uint64_t hit = __ballot(found >= 0), some = __ballot(seen >= 0);
+                        const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
+                        if (lane == l) sh_at = seen, sh_count = fc, sh_sum = fw, sh_ties = fn;
+                    }
+                    __syncthreads();
+                    before_c += sh_count;
+                    before_w += (double)sh_sum;
+                    equal = sh_ties;
+                    prefix = (prefix << width) | (uint32_t)sh_at;
+                }
+                key = (prefix << low_bit) | rest;
+            }
+            // the ties of `key` that are kept, before_c entries or before_w of weight lying above them
+            const uint64_t w = scale.weight(key);
+            if (by_count) {
+                const int64_t left = count - before_c;
+                ties = left < (int64_t)equal ? (uint32_t)left : equal;
+            } else {
+                uint32_t lo = 1, hi = equal;             // the fewest that reach the target
+                while (lo < hi) {
+                    const uint32_t mid = (lo + hi) / 2;
+                    if (before_w + (double)(mid * w) >= target) hi = mid;
+                    else lo = mid + 1;
+                }
+                ties = lo;
+            }
+            total = before_w + (double)(ties * w);
+            have_total = true;
         }
     }
+    const uint32_t lowest = key > min_key ? key : min_key;
     // ---- the index of the last tie that is kept ----------------------------------------------------------------------------
     int last = a.V;
-    if (ties < equal) {
+    if (!LOCAL && listed && ties < equal && key >= lowest) {
+        // all entries equal to `key` are in the list: the one with ties - 1 of them before it
+        uint32_t *const same = reinterpret_cast<uint32_t *>(seg_w);
+        static_assert(LOCAL || sizeof(seg_w) >= kList * sizeof(uint32_t), "room for their indexes");
         __syncthreads();
-        for_groups([&](const uint32_t (&k)[8], uint32_t have, int, int s) {
+        if (tid == 0) sh_n = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < list_n; i += THREADS)
+            if (list[i].key == key) same[atomicAdd(&sh_n, 1u)] = (uint32_t)list[i].index;
+        __syncthreads();
+        const uint32_t n = sh_n;
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const uint32_t mine = same[i];
+            uint32_t before = 0;
+#pragma unroll 8
+            for (uint32_t j = 0; j < n; j++) before += same[j] < mine;
+            if (before == ties - 1) sh_at = (int)mine;
+        }
+        __syncthreads();
+        last = sh_at;
+    } else if (ties < equal && key >= lowest) {
+        __syncthreads();
+        for_groups(one_ahead, 0, segs, [&](const uint32_t (&k)[8], uint32_t have, int, int s) {
             uint32_t c = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) c += (have >> e & 1) && k[e] == key;
             c = wave_sum(c);
-            if (lane == 0) seg_c[s] = c;
+            if (lane == 0) seg_w[s] = c;
         });
         __syncthreads();
         if (wave == 0) {
             uint32_t left = ties;                        // among the segments from base on
             int base = 0;
             for (;; base += 64) {
-                const uint32_t c = base + lane < segs ? seg_c[base + lane] : 0;
+                const uint32_t c = base + lane < segs ? (uint32_t)seg_w[base + lane] : 0;
                 const uint32_t run = wave_scan(c, lane);
                 const uint64_t hit = __ballot(run >= left);
                 if (hit || base + 64 >= segs) {
@@ -653,6 +1001,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
             const uint64_t hit = __ballot(run >= left);
             if (hit && lane == __builtin_ctzll(hit)) {
                 left -= run - c;
+#pragma unroll
                 for (int e = 0; e < 8; e++)
                     if ((have >> e & 1) && --left == 0) sh_at = j * kGroup - x.lead + e;
             }
@@ -661,81 +1010,45 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
         last = sh_at;
     }
     // ---- the draw ----------------------------------------------------------------------------------------------------------
-    const double min_w = std::min(set.min_p, 1.0) * one;
-    // no entry below this reaches min_p (a little lower than it need be; the weights decide)
-    uint32_t lowest = set.min_p > 0.0 ? TokenKey<T>::below(scale.vmax + log2(std::min(set.min_p, 1.0)) / set.rate) : 0u;
-    lowest = lowest > key ? lowest : key;
-    const auto draw = [&](const TokenScale<T> &sc, int seg0, int seg1, auto &&bar_of) {
-        const auto kept = [&](uint32_t k, int i) -> uint64_t {
-            if (k < lowest || (k == key && i > last)) return 0;
-            const uint64_t w = sc.weight(k);
-            return (double)w < min_w ? 0 : w;
-        };
-        __syncthreads();
-        for (int s = seg0 + wave; s < seg1; s += WAVES) {
-            uint32_t k[8], have = 0;
-            const int j = s * kSegGroups + lane;
-            if (j < x.groups) have = x.load(k, j);
-            uint64_t w = 0;
-            for (int e = 0; e < 8; e++)
-                if (have >> e & 1) w += kept(k[e], j * kGroup - x.lead + e);
-            w = wave_sum(w);
-            if (lane == 0) seg_w[s] = w;
-        }
-        __syncthreads();
-        if (wave != 0) return;
-        uint64_t all = 0;
-        for (int s = seg0 + lane; s < seg1; s += 64) all += seg_w[s];
-        all = wave_sum(all);
-        uint64_t bar = bar_of(all);                      // below all: some segment reaches over it
-        int base = seg0;
-        for (;; base += 64) {
-            const uint64_t c = base + lane < seg1 ? seg_w[base + lane] : 0;
-            const uint64_t run = wave_scan(c, lane);
-            const uint64_t hit = __ballot(run > bar);
-            if (hit || base + 64 >= seg1) {
-                const int l = hit ? __builtin_ctzll(hit) : 63;
-                bar -= __shfl(run, l) - __shfl(c, l);
-                base += l;
-                break;
-            }
-            bar -= __shfl(run, 63);
-        }
-        uint32_t k[8], have = 0;
-        uint64_t w[8], sum = 0;
-        const int j = base * kSegGroups + lane;
-        if (j < x.groups) have = x.load(k, j);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            w[e] = have >> e & 1 ? kept(k[e], j * kGroup - x.lead + e) : 0;
-            sum += w[e];
-        }
-        const uint64_t run = wave_scan(sum, lane);
-        const uint64_t hit = __ballot(run > bar);
-        if (hit && lane == __builtin_ctzll(hit)) {
-            uint64_t acc = run - sum;
-            int i = -1;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                acc += w[e];
-                if (i < 0 && acc > bar) i = j * kGroup - x.lead + e;
-            }
-            a.out[row] = i;
-        }
-    };
+    const auto passes = [&](uint32_t k, int i) { return k >= lowest && (k != key || i <= last); };
     const uint32_t word = a.words[row];
+    int seg0 = 0, seg1 = segs;                           // where the token lies
+    uint32_t drawn_max = m;                              // what the weights are relative to there
+    bool by_chunks = false;
     if constexpr (!LOCAL) {
-        if (!set.cut() && !(set.min_p > 0.0)) {
-            // nothing is cut off: the chunk from the chunks' sums, then that chunk's entries alone
+        // The chunk first.  What is kept of every one: of the slots above the border's all, which its histogram holds, of the
+        // border's slot the entries of the list.
+        by_chunks = border == kSlots || listed;
+        if (by_chunks && border < kSlots) {
+            for (int c = wave; c < a.chunks; c += WAVES) {
+                uint64_t w = 0;
+                const int below = border - chunk_off[c];             // the chunk's slots above the row's border
+#pragma unroll
+                for (int q = 0; q < kSlots / 64; q++)
+                    if (q * 64 + lane < below) w += chunk[c].weight[q * 64 + lane];
+                w = wave_sum(w);
+                if (lane == 0) chunk_w[c] = w;
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < list_n; i += THREADS) {
+                const TokenEntry q = list[i];
+                if (!passes(q.key, q.index)) continue;
+                const int c = (q.index + x.lead) / (kGroup * kChunkGroups);
+                const TokenScale<T> sc(chunk[c].kmax, set.rate, a.frac_bits, &table);
+                atomicAdd((unsigned long long *)&chunk_w[c], (unsigned long long)sc.weight(q.key));
+            }
+        }
+        if (by_chunks) {
+            __syncthreads();
             if (wave == 0) {
                 double all = 0.0, before = 0.0;
                 for (int c0 = 0; c0 < a.chunks; c0 += 64)
-                    all += wave_sum(c0 + lane < a.chunks ? chunk_f[c0 + lane] * (double)chunk[c0 + lane].sum : 0.0);
+                    all += wave_sum(c0 + lane < a.chunks ? chunk_f[c0 + lane] * (double)chunk_w[c0 + lane] : 0.0);
                 const double bar = (double)word * 0x1p-32 * all;
                 int at = -1, seen = -1;                  // the chunk that reaches over the bar; the last with any weight
                 double from = 0.0;
                 for (int c0 = 0; c0 < a.chunks && at < 0; c0 += 64) {
-                    const double v = c0 + lane < a.chunks ? chunk_f[c0 + lane] * (double)chunk[c0 + lane].sum : 0.0;
+                    const double v = c0 + lane < a.chunks ? chunk_f[c0 + lane] * (double)chunk_w[c0 + lane] : 0.0;
                     const double run = wave_scan(v, lane);
                     const uint64_t hit = __ballot(v > 0.0 && before + run > bar), some = __ballot(v > 0.0);
                     const int l = hit ? __builtin_ctzll(hit) : some ? 63 - __builtin_clzll(some) : -1;
@@ -750,18 +1063,69 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                 if (lane == 0) sh_at = at, sh_before = (bar - from) / chunk_f[at];
             }
             __syncthreads();
-            const int at = sh_at;
-            const double left = sh_before;
             constexpr int kSegsPerChunk = kChunkGroups / kSegGroups;
-            const int seg1 = (at + 1) * kSegsPerChunk < segs ? (at + 1) * kSegsPerChunk : segs;
-            draw(TokenScale<T>(chunk[at].kmax, set.rate, a.frac_bits), at * kSegsPerChunk, seg1, [&](uint64_t all) {
-                const uint64_t b = left > 0.0 ? (uint64_t)left : 0;
-                return b < all ? b : all - 1;
-            });
-            return;
+            seg0 = sh_at * kSegsPerChunk;
+            seg1 = seg0 + kSegsPerChunk < segs ? seg0 + kSegsPerChunk : segs;
+            drawn_max = chunk[sh_at].kmax;
         }
     }
-    draw(scale, 0, segs, [&](uint64_t all) { return token_bar(word, all); });
+    const TokenScale<T> drawn(drawn_max, set.rate, a.frac_bits, &table);
+    const auto kept = [&](uint32_t k, int i, bool have) -> uint64_t {
+        return have && passes(k, i) ? drawn.weight(k) : 0;
+    };
+    __syncthreads();
+    for_groups(one_ahead, seg0, seg1, [&](const uint32_t (&k)[8], uint32_t have, int i0, int s) {
+        uint64_t w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) w += kept(k[e], i0 + e, have >> e & 1);
+        w = wave_sum(w);
+        if (lane == 0) seg_w[s] = w;
+    });
+    __syncthreads();
+    if (wave != 0) return;
+    uint64_t all = 0;
+    for (int s = seg0 + lane; s < seg1; s += 64) all += seg_w[s];
+    all = wave_sum(all);
+    uint64_t bar = token_bar(word, all);                 // below all: some segment reaches over it
+    if (by_chunks) {
+        const double left = sh_before;
+        bar = left > 0.0 ? (uint64_t)left : 0;
+        bar = bar < all ? bar : all - 1;
+    }
+    int base = seg0;
+    for (;; base += 64) {
+        const uint64_t c = base + lane < seg1 ? seg_w[base + lane] : 0;
+        const uint64_t run = wave_scan(c, lane);
+        const uint64_t hit = __ballot(run > bar);
+        if (hit || base + 64 >= seg1) {
+            const int l = hit ? __builtin_ctzll(hit) : 63;
+            bar -= __shfl(run, l) - __shfl(c, l);
+            base += l;
+            break;
+        }
+        bar -= __shfl(run, 63);
+    }
+    uint32_t k[8], have = 0;
+    uint64_t w[8], sum = 0;
+    const int j = base * kSegGroups + lane;
+    if (j < x.groups) have = x.load(k, j);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        w[e] = kept(k[e], j * kGroup - x.lead + e, have >> e & 1);
+        sum += w[e];
+    }
+    const uint64_t run = wave_scan(sum, lane);
+    const uint64_t hit = __ballot(run > bar);
+    if (hit && lane == __builtin_ctzll(hit)) {
+        uint64_t acc = run - sum;
+        int i = -1;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            acc += w[e];
+            if (i < 0 && acc > bar) i = j * kGroup - x.lead + e;
+        }
+        a.out[row] = i;
+    }
 }
 
 static int token_chunks(int64_t V) { return (int)ceil_div(V + kGroup - 1, kChunkGroups * kGroup); }
@@ -771,14 +1135,16 @@ static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
 {
     if (a.V <= 64)
         sample_short_kernel<T><<<dim3((unsigned)ceil_div(a.R, 4)), dim3(256), 0, st>>>(a);
-    else if (a.V <= 2048)
-        sample_row_kernel<T, 256, true><<<dim3((unsigned)a.R), dim3(256), 0, st>>>(a);
+    else if (a.V <= 256 * kGroup - 8)                    // a row that starts inside a group reaches into one more
+        sample_row_kernel<T, 256, 1><<<dim3((unsigned)a.R), dim3(256), 0, st>>>(a);
+    else if (a.V <= 1024 * kGroup - 8)
+        sample_row_kernel<T, 1024, 1><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
     else if (a.V <= kTokenLocalV)
-        sample_row_kernel<T, 1024, true><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
+        sample_row_kernel<T, 1024, 2><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
     else {
-        token_chunk_kernel<T><<<dim3((unsigned)(a.R * a.chunks)), dim3(512), 0, st>>>(a);
+        token_chunk_kernel<T><<<dim3((unsigned)std::min<int64_t>(a.R * a.chunks, kChunkGrid)), dim3(512), 0, st>>>(a);
         if (const int rc = check_launch(who)) return rc;
-        sample_row_kernel<T, 1024, false><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
+        sample_row_kernel<T, 1024, 0><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
     }
     return check_launch(who);
 }
@@ -826,7 +1192,7 @@ int nb_sample_tokens(int32_t *out, const void *logits, int type, const uint32_t 
     int log2v = 0;
     while ((1LL << log2v) < V) log2v++;
     const nb::TokenArgs a{out, logits, words, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all,
-                          top_k_all, R, (int)V, std::min(52, 61 - log2v), nb::token_chunks(V), (uint8_t *)workspace};
+                          top_k_all, R, (int)V, std::min(51, 61 - log2v), nb::token_chunks(V), (uint8_t *)workspace};
     const hipStream_t st = nb::as_stream(stream);
     if (type == NB_TYPE_F32) return nb::token_launch<float>(a, st, who);
     if (type == NB_TYPE_F16) return nb::token_launch<_Float16>(a, st, who);

@@ -97,7 +97,7 @@ def mm_nt(a, b):
 
 def sample(logits, word, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One row (float64 logits) -> token.  Weights are whole multiples of 2^-f, as the format of the operator says: f =
-    min(52, 61 - ceil(log2 V)) fraction bits; those below half a unit are 0.  (All of a row's zeros together stand for less
+    min(51, 61 - ceil(log2 V)) fraction bits; those below half a unit are 0.  (All of a row's zeros together stand for less
     than V 2^-(f+1) of the largest weight: 2^-28 at V = 131072 and at V <= 2^14 less than 2^-32, which only a word of 0 could
     ask for.)"""
     x = [float(v) for v in logits]
@@ -109,7 +109,7 @@ def sample(logits, word, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not temperature > 0:
         return order[0]
 
-    unit = 2 ** min(52, 61 - math.ceil(math.log2(len(x))))
+    unit = 2 ** min(51, 61 - math.ceil(math.log2(len(x))))
 
     def weight(i):
         if x[i] == top:
