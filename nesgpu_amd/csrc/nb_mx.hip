@@ -85,20 +85,92 @@ __device__ __forceinline__ void mx_load_weight8(float (&w)[8], RowWeight weight,
         mx_load_row8<VEC>(w, (const Bf16 *)weight.p, k0, K);
 }
 
-__device__ __forceinline__ float mx_round(float v, float) { return v; }
-__device__ __forceinline__ float mx_round(float v, _Float16) { return (float)(_Float16)v; }
-__device__ __forceinline__ float mx_round(float v, Bf16) { return __builtin_bit_cast(float, (uint32_t)mx_bf16(v) << 16); }
-
-template <bool VEC, typename T, typename R>
-__device__ __forceinline__ void norm_input(float (&h)[8], const T *x, const R *residual, int64_t k0, int64_t K)
-{
-    mx_load_row8<VEC>(h, x, k0, K);
-    if constexpr (!__is_same(R, NoType)) {
-        float r[8];
-        mx_load_row8<VEC>(r, residual, k0, K);
+// Eight elements of a row as they lie in memory.  Loads leave them so, and the conversions come after: a row's loads are all
+// under way together (converted one by one where they are loaded, the second of 8192 x 8192 rows in bf16 waits for the
+// first), and 16-bit values keep to half the registers between the sum and the products.
+template <typename T>
+struct MxRaw {
+    uint32_t w[sizeof(T) == 2 ? 4 : 8] = {};
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T *row, int64_t k0, int64_t K)   // zeros past the row's end
+    {
+        if (VEC ? k0 < K : k0 + 8 <= K) {
+            const auto *q = reinterpret_cast<const mx_words<VEC, T> *>(row + k0);
 #pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = mx_round(h[i] + r[i], R{});
+            for (int j = 0; j < (sizeof(T) == 2 ? 1 : 2); j++) {
+                const auto a = q[j];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[4 * j + i] = a[i];
+            }
+        } else if (!VEC) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (k0 + i < K) {
+                    if constexpr (sizeof(T) == 2)
+                        w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[k0 + i]) << (16 * (i & 1));
+                    else
+                        w[i] = __builtin_bit_cast(uint32_t, row[k0 + i]);
+                }
+        }
     }
+    __device__ __forceinline__ void set(int i, float v)                          // rounds; i upwards from a cleared start
+    {
+        if constexpr (__is_same(T, Bf16))
+            w[i / 2] = i & 1 ? w[i / 2] | (uint32_t)mx_bf16(v) << 16 : mx_bf16(v);
+        else if constexpr (__is_same(T, _Float16))
+            w[i / 2] = i & 1 ? w[i / 2] | (uint32_t)mx_f16(v) << 16 : mx_f16(v);
+        else
+            w[i] = __builtin_bit_cast(uint32_t, v);
+    }
+    __device__ __forceinline__ float get(int i) const
+    {
+        if constexpr (sizeof(T) == 2)
+            return mx_float(w[i / 2], i & 1, T{});
+        else if constexpr (__is_same(T, int32_t))
+            return (float)(int32_t)w[i];
+        else
+            return __builtin_bit_cast(float, w[i]);
+    }
+};
+// what is normalised: the rows themselves or, with a residual, the sums rounded to its type
+template <typename X, typename R>
+struct MxHeldAs {
+    typedef R type;
+};
+template <typename X>
+struct MxHeldAs<X, NoType> {
+    typedef X type;
+};
+template <bool VEC, int N, typename H, typename X, typename R>
+__device__ __forceinline__ void norm_input(MxRaw<H> (&h)[N], const X *x, const R *residual, int64_t p, int64_t T, int64_t K)
+{
+    if constexpr (__is_same(R, NoType)) {
+#pragma unroll
+        for (int j = 0; j < N; j++) h[j].template load<VEC>(x, 8 * (p + T * j), K);
+    } else {
+        MxRaw<X> a[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            a[j].template load<VEC>(x, 8 * (p + T * j), K);
+            h[j].template load<VEC>(residual, 8 * (p + T * j), K);
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = a[j].get(i) + h[j].get(i);
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[j].set(i, v[i]);
+        }
+    }
+}
+template <bool VEC, typename H>
+__device__ __forceinline__ void norm_store(H *row, int64_t k0, int64_t K, const MxRaw<H> &h)
+{
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = h.get(i);
+    mx_store_row8<VEC>(row, k0, K, v);
 }
 
 template <int T>
@@ -117,13 +189,22 @@ __device__ __forceinline__ double row_sum(double s, double *part)
 }
 
 // T threads per row (a workgroup, or for T = 64 a wave of a workgroup of four rows).  N > 0: the row (at most 8 T N
-// elements) stays in registers between the two uses; N = 0: rows of any length, read twice.
+// elements) stays in registers between the sum and the products; N = 0: rows of any length, read again for the products,
+// out of the caches for the most part.
+//
+// Bound by memory: with a residual in bf16 7 + 1/32 bytes an element, 8192 x 8192 in 92 to 102 us (4.6 to 5.1 TB/s; a large copy
+// 5.1).  The weights are loaded after the sum: taken before it they cost 16 registers per piece over the barrier and a
+// third of the waves (151 us).  Without a residual the 64-bit products show: 58 us for 3.0 bytes an element, 3.5 TB/s.
+// One piece per thread: 8 waves a SIMD (64 registers) 16384 x 4096 90 us, 95 with 68 registers; two pieces need their 92.
+// Rows above 8192 are read twice: 4096 x 16384 bf16 105 us (held by 1024 threads of two pieces 107), 2000 x 32000 fp16
+// 107 us (of four pieces 131), 3355 x 20001 fp32 215 us (219).
 template <typename X, typename R, bool FP8, bool VEC, int T, int N>
-__global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_mx_kernel(uint8_t *codes, uint8_t *scales, R *residual_out,
+__global__ __launch_bounds__(T == 64 ? 256 : T, N == 1 ? 8 : 1) void rms_norm_mx_kernel(uint8_t *codes, uint8_t *scales, R *residual_out,
                                                                       const X *x, const R *residual, RowWeight weight,
                                                                       double eps, int64_t rows, int64_t K,
                                                                       int64_t row_pieces)
 {
+    typedef typename MxHeldAs<X, R>::type H;
     __shared__ double part[T / 64 + 1];
     constexpr int kRows = T == 64 ? 4 : 1;
     const int tid = T == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
@@ -133,45 +214,49 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_mx_kernel(uint8_t 
         const R *rr = residual;
         R *ro = residual_out;
         if constexpr (!__is_same(R, NoType)) rr += row * K, ro += row * K;
-        constexpr int kHeld = N > 0 ? N : 1;
-        float h[kHeld][8];
+        const int64_t out0 = row * row_pieces;
         double s = 0.0;
-        if (N > 0) {
+        if constexpr (N > 0) {
+            MxRaw<H> h[N];
+            norm_input<VEC>(h, xr, rr, tid, T, K);
 #pragma unroll
-            for (int j = 0; j < kHeld; j++) norm_input<VEC>(h[j], xr, rr, 8 * (tid + (int64_t)T * j), K);
+            for (int j = 0; j < N; j++) {
+                if constexpr (!__is_same(R, NoType)) norm_store<VEC>(ro, 8 * (tid + (int64_t)T * j), K, h[j]);
 #pragma unroll
-            for (int j = 0; j < kHeld; j++) {
-                if constexpr (!__is_same(R, NoType)) mx_store_row8<VEC>(ro, 8 * (tid + (int64_t)T * j), K, h[j]);
+                for (int i = 0; i < 8; i++) s = fma((double)h[j].get(i), (double)h[j].get(i), s);
+            }
+            s = row_sum<T>(s, part);
+            const double r = 1.0 / sqrt(s / (double)K + eps);
 #pragma unroll
-                for (int i = 0; i < 8; i++) s = fma((double)h[j][i], (double)h[j][i], s);
+            for (int j = 0; j < N; j++) {
+                const int64_t p = tid + (int64_t)T * j;
+                float w[8], v[8];
+                mx_load_weight8<VEC>(w, weight, 8 * p, K);
+                if (p < row_pieces) {                    // whole blocks: row_pieces and T are multiples of 4
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = 8 * p < K ? (float)(((double)h[j].get(i) * r) * (double)w[i]) : 0.f;
+                    mx_emit8<FP8>(codes, scales, out0 + p, v);
+                }
             }
         } else {
-            for (int64_t p = tid; 8 * p < K; p += T) {
-                norm_input<VEC>(h[0], xr, rr, 8 * p, K);
+            for (int64_t p = tid; 8 * p < K; p += 2 * T) {
+                MxRaw<H> h[2];
+                norm_input<VEC>(h, xr, rr, p, T, K);
 #pragma unroll
-                for (int i = 0; i < 8; i++) s = fma((double)h[0][i], (double)h[0][i], s);
+                for (int i = 0; i < 16; i++) s = fma((double)h[i / 8].get(i % 8), (double)h[i / 8].get(i % 8), s);
             }
-        }
-        s = row_sum<T>(s, part);
-        const double r = 1.0 / sqrt(s / (double)K + eps);
-        const int64_t out0 = row * row_pieces;
-        for (int64_t p = tid, j = 0; p < row_pieces; p += T, j++) {
-            float v[8], w[8];
-            mx_load_weight8<VEC>(w, weight, 8 * p, K);
-            if (N > 0) {
+            s = row_sum<T>(s, part);
+            const double r = 1.0 / sqrt(s / (double)K + eps);
+            for (int64_t p = tid; p < row_pieces; p += T) {
+                float v[8], w[8];
+                MxRaw<H> h[1];
+                norm_input<VEC>(h, xr, rr, p, 0, K);
+                mx_load_weight8<VEC>(w, weight, 8 * p, K);
+                if constexpr (!__is_same(R, NoType)) norm_store<VEC>(ro, 8 * p, K, h[0]);
 #pragma unroll
-                for (int q = 0; q < kHeld; q++)
-                    if (q == (int)j) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = h[q][i];
-                    }
-            } else {
-                norm_input<VEC>(v, xr, rr, 8 * p, K);
-                if constexpr (!__is_same(R, NoType)) mx_store_row8<VEC>(ro, 8 * p, K, v);
+                for (int i = 0; i < 8; i++) v[i] = 8 * p < K ? (float)(((double)h[0].get(i) * r) * (double)w[i]) : 0.f;
+                mx_emit8<FP8>(codes, scales, out0 + p, v);
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 8 * p < K ? (float)(((double)v[i] * r) * (double)w[i]) : 0.f;
-            mx_emit8<FP8>(codes, scales, out0 + p, v);
         }
         if (T > 64) __syncthreads();   // part[] is free for the next row
     }
@@ -243,10 +328,10 @@ static void norm_launch_vec(const NormArgs &a)
         norm_launch_n<X, R, FP8, VEC, 64, 1>(a);
     else if (Kp <= 256 * 8)
         norm_launch_n<X, R, FP8, VEC, 256, 1>(a);
-    else if (Kp <= 256 * 16)
-        norm_launch_n<X, R, FP8, VEC, 256, 2>(a);
-    else if (Kp <= 256 * 32)
-        norm_launch_n<X, R, FP8, VEC, 256, 4>(a);
+    else if (Kp <= 512 * 8)
+        norm_launch_n<X, R, FP8, VEC, 512, 1>(a);
+    else if (Kp <= 512 * 16)
+        norm_launch_n<X, R, FP8, VEC, 512, 2>(a);
     else
         norm_launch_n<X, R, FP8, VEC, 1024, 0>(a);
 }

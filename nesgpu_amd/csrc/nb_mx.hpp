@@ -22,18 +22,25 @@ struct Bf16 {
     uint16_t bits;
 };
 
-// 8 consecutive elements at p (16-byte aligned) as floats; int32 is converted (exact up to 2^24).
-__device__ __forceinline__ void mx_load8(float (&v)[8], const float *p)
-{
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void mx_load8(float (&v)[8], const int32_t *p)
-{
-    const int4 a = reinterpret_cast<const int4 *>(p)[0], b = reinterpret_cast<const int4 *>(p)[1];
-    v[0] = (float)a.x, v[1] = (float)a.y, v[2] = (float)a.z, v[3] = (float)a.w;
-    v[4] = (float)b.x, v[5] = (float)b.y, v[6] = (float)b.z, v[7] = (float)b.w;
-}
+// 16 bytes at an address that is a multiple of ALIGN only.  The hardware reads and writes memory at any multiple of 2 or 4
+// bytes; rows of odd length keep their wide accesses.
+template <int ALIGN>
+struct MxWords;
+template <>
+struct MxWords<16> {
+    typedef uint32_t type __attribute__((ext_vector_type(4)));
+};
+template <>
+struct MxWords<4> {
+    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct MxWords<2> {
+    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <bool VEC, typename T>
+using mx_words = typename MxWords<VEC ? 16 : (int)sizeof(T)>::type;
+
 __device__ __forceinline__ float mx_float(uint32_t w, int half, _Float16)
 {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(half ? w >> 16 : w & 0xFFFFu));
@@ -42,56 +49,66 @@ __device__ __forceinline__ float mx_float(uint32_t w, int half, Bf16)
 {
     return __builtin_bit_cast(float, half ? w & 0xFFFF0000u : w << 16);
 }
-template <typename T16>
-__device__ __forceinline__ void mx_load8(float (&v)[8], const T16 *p)
+// 8 consecutive elements at p as floats (VEC: 16-byte aligned); int32 is converted (exact up to 2^24)
+template <bool VEC = true, typename T>
+__device__ __forceinline__ void mx_load8(float (&v)[8], const T *p)
 {
-    const uint4 a = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    const auto *q = reinterpret_cast<const mx_words<VEC, T> *>(p);
+    if constexpr (sizeof(T) == 4) {
+        const auto a = q[0], b = q[1];
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[2 * i] = mx_float(w[i], 0, T16{}), v[2 * i + 1] = mx_float(w[i], 1, T16{});
+        for (int i = 0; i < 4; i++) {
+            if constexpr (__is_same(T, int32_t))
+                v[i] = (float)(int32_t)a[i], v[4 + i] = (float)(int32_t)b[i];
+            else
+                v[i] = __builtin_bit_cast(float, (uint32_t)a[i]), v[4 + i] = __builtin_bit_cast(float, (uint32_t)b[i]);
+        }
+    } else {
+        const auto a = q[0];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[2 * i] = mx_float(a[i], 0, T{}), v[2 * i + 1] = mx_float(a[i], 1, T{});
+    }
 }
 __device__ __forceinline__ float mx_load1(const float *p) { return *p; }
 __device__ __forceinline__ float mx_load1(const int32_t *p) { return (float)*p; }
 __device__ __forceinline__ float mx_load1(const _Float16 *p) { return (float)*p; }
 __device__ __forceinline__ float mx_load1(const Bf16 *p) { return __builtin_bit_cast(float, (uint32_t)p->bits << 16); }
-// elements k0 .. k0 + 7 of a row of K, zeros past its end; VEC: k0 + 8 <= K or k0 >= K, and the address is aligned
+// elements k0 .. k0 + 7 of a row of K, zeros past its end; VEC: K is a multiple of 8 and the address aligned
 template <bool VEC, typename T>
 __device__ __forceinline__ void mx_load_row8(float (&v)[8], const T *row, int64_t k0, int64_t K)
 {
-    if (VEC) {
-        if (k0 < K) {
-            mx_load8(v, row + k0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 0.f;
-        }
+    if (VEC ? k0 < K : k0 + 8 <= K) {
+        mx_load8<VEC>(v, row + k0);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = k0 + i < K ? mx_load1(row + k0 + i) : 0.f;
+        for (int i = 0; i < 8; i++) v[i] = !VEC && k0 + i < K ? mx_load1(row + k0 + i) : 0.f;
     }
 }
 
 // fp32 -> the stored types, to nearest, ties to even
 __device__ __forceinline__ uint16_t mx_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 __device__ __forceinline__ uint16_t mx_f16(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
-__device__ __forceinline__ void mx_store8(float *p, const float (&v)[8])
+template <bool VEC = true, typename T>
+__device__ __forceinline__ void mx_store8(T *p, const float (&v)[8])
 {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void mx_store8(_Float16 *p, const float (&v)[8])
-{
-    uint32_t w[4];
+    auto *q = reinterpret_cast<mx_words<VEC, T> *>(p);
+    if constexpr (sizeof(T) == 4) {
+        mx_words<VEC, T> a, b;
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = mx_f16(v[2 * i]) | ((uint32_t)mx_f16(v[2 * i + 1]) << 16);
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void mx_store8(Bf16 *p, const float (&v)[8])
-{
-    uint32_t w[4];
+        for (int i = 0; i < 4; i++)
+            a[i] = __builtin_bit_cast(uint32_t, v[i]), b[i] = __builtin_bit_cast(uint32_t, v[4 + i]);
+        q[0] = a, q[1] = b;
+    } else {
+        mx_words<VEC, T> a;
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = mx_bf16(v[2 * i]) | ((uint32_t)mx_bf16(v[2 * i + 1]) << 16);
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 4; i++) {
+            if constexpr (__is_same(T, Bf16))
+                a[i] = mx_bf16(v[2 * i]) | ((uint32_t)mx_bf16(v[2 * i + 1]) << 16);
+            else
+                a[i] = mx_f16(v[2 * i]) | ((uint32_t)mx_f16(v[2 * i + 1]) << 16);
+        }
+        q[0] = a;
+    }
 }
 __device__ __forceinline__ void mx_store1(float *p, float v) { *p = v; }
 __device__ __forceinline__ void mx_store1(_Float16 *p, float v) { *p = (_Float16)v; }
@@ -99,9 +116,9 @@ __device__ __forceinline__ void mx_store1(Bf16 *p, float v) { p->bits = mx_bf16(
 template <bool VEC, typename T>
 __device__ __forceinline__ void mx_store_row8(T *row, int64_t k0, int64_t K, const float (&v)[8])
 {
-    if (VEC) {
-        if (k0 < K) mx_store8(row + k0, v);
-    } else {
+    if (VEC ? k0 < K : k0 + 8 <= K) {
+        mx_store8<VEC>(row + k0, v);
+    } else if (!VEC) {
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (k0 + i < K) mx_store1(row + k0 + i, v[i]);
