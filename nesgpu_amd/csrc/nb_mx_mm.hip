@@ -59,7 +59,7 @@ __device__ __forceinline__ void mx_split(mx_v8i &lo, mx_v8i &hi, mx_v4i a0, mx_v
 }
 
 // ---- few rows: one operand is streamed, fragments straight from memory ------------------------------------------------
-// A workgroup makes one tile of 16 MT x 16 NT outputs; its W waves take every W-th chunk of four steps, and their sums
+// A workgroup makes one tile of rm MT x rn NT outputs (rm, rn <= 16); its W waves take every W-th chunk of four steps, and their sums
 // meet in shared memory in a fixed order.  What bounds it is the number of row pieces per load, about 4 cycles each
 // whatever their size: a fragment load has 16 of 64 bytes, and a load of one scale dword per row would cost as much again,
 // so a row's four scale dwords of a chunk come in one load (where they are aligned; else one by one).
@@ -67,7 +67,7 @@ template <bool FP8, typename O, int MT, int NT, int W>
 __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, const uint8_t *__restrict__ A,
                                                             const uint32_t *__restrict__ As, const uint8_t *__restrict__ B,
                                                             const uint32_t *__restrict__ Bs, int64_t M, int64_t N,
-                                                            int64_t steps, int64_t ntiles, bool whole)
+                                                            int64_t steps, int64_t ntiles, bool whole, int rm, int rn)
 {
     constexpr int ABYTES = FP8 ? 128 : 64;
     __shared__ float part[W][MT * NT][256];
@@ -75,15 +75,18 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
     const int64_t mt = blockIdx.x / ntiles, nt = blockIdx.x - mt * ntiles;
     const uint8_t *a[MT], *b[NT];
     const uint32_t *as[MT], *bs[NT];
+    bool in_a[MT], in_b[NT];                             // lanes without a row load nothing and supply zeros
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-        const int64_t m = std::min<int64_t>(16 * (mt * MT + i) + r16, M - 1);   // rows past the end: the last one again
+        const int64_t m = rm * (mt * MT + i) + r16;
+        in_a[i] = r16 < rm && m < M;
         a[i] = A + m * steps * ABYTES;
         as[i] = As + m * steps;
     }
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-        const int64_t n = std::min<int64_t>(16 * (nt * NT + j) + r16, N - 1);
+        const int64_t n = rn * (nt * NT + j) + r16;
+        in_b[j] = r16 < rn && n < N;
         b[j] = B + n * steps * 64;
         bs[j] = Bs + n * steps;
     }
@@ -98,15 +101,17 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
     };
     const int64_t chunks = steps >> 2;
     for (int64_t c = wave; c < chunks; c += W) {
-        mx_v4i fb[NT][4], fa[MT][4][FP8 ? 2 : 1], sb[NT], sa[MT];
+        mx_v4i fb[NT][4] = {}, fa[MT][4][FP8 ? 2 : 1] = {}, sb[NT] = {}, sa[MT] = {};
 #pragma unroll
         for (int j = 0; j < NT; j++) {
+            if (!in_b[j]) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) fb[j][e] = *reinterpret_cast<const mx_v4i *>(b[j] + (4 * c + e) * 64 + 16 * g);
             sb[j] = scales4(bs[j] + 4 * c);
         }
 #pragma unroll
         for (int i = 0; i < MT; i++) {
+            if (!in_a[i]) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint8_t *p = a[i] + (4 * c + e) * ABYTES + 16 * g;
@@ -128,15 +133,27 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
             }
     }
     for (int64_t s = 4 * chunks + wave; s < steps; s += W) {
+        mx_v4i fb[NT] = {}, fa[MT][FP8 ? 2 : 1] = {};
+        uint32_t sb[NT] = {}, sa[MT] = {};
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+            if (in_b[j]) {
+                fb[j] = *reinterpret_cast<const mx_v4i *>(b[j] + s * 64 + 16 * g);
+                sb[j] = bs[j][s];
+            }
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            const uint8_t *p = a[i] + s * ABYTES + 16 * g;
+            if (in_a[i]) {
+                const uint8_t *p = a[i] + s * ABYTES + 16 * g;
+                fa[i][0] = *reinterpret_cast<const mx_v4i *>(p);
+                if (FP8) fa[i][FP8 ? 1 : 0] = *reinterpret_cast<const mx_v4i *>(p + 64);
+                sa[i] = as[i][s];
+            }
             mx_v8i lo, hi;
-            mx_split<FP8>(lo, hi, *reinterpret_cast<const mx_v4i *>(p), *reinterpret_cast<const mx_v4i *>(p + (FP8 ? 64 : 0)));
-            const int sa = (int)(as[i][s] >> (8 * g));
+            mx_split<FP8>(lo, hi, fa[i][0], fa[i][FP8 ? 1 : 0]);
 #pragma unroll
             for (int j = 0; j < NT; j++)
-                mx_step<FP8>(acc[i][j], lo, hi, mx_frag4(b[j] + s * 64 + 16 * g), sa, (int)(bs[j][s] >> (8 * g)));
+                mx_step<FP8>(acc[i][j], lo, hi, mx_wide(fb[j]), (int)(sa[i] >> (8 * g)), (int)(sb[j] >> (8 * g)));
         }
     }
 #pragma unroll
@@ -150,9 +167,9 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < W; w++) v += part[w][t >> 8][t & 255];
-        const int64_t m = 16 * (mt * MT + (t >> 8) / NT) + ((t & 255) >> 4);
-        const int64_t n = 16 * (nt * NT + (t >> 8) % NT) + (t & 15);
-        if (m < M && n < N) mx_store1(C + m * N + n, v);
+        const int rt = (t & 255) >> 4, ct = t & 15;
+        const int64_t m = rm * (mt * MT + (t >> 8) / NT) + rt, n = rn * (nt * NT + (t >> 8) % NT) + ct;
+        if (rt < rm && ct < rn && m < M && n < N) mx_store1(C + m * N + n, v);
     }
 }
 
@@ -435,12 +452,12 @@ static int mm_tile_launch(const MmArgs &a, const char *who)
 }
 
 template <bool FP8, typename O, int MT, int NT, int W>
-static int mm_rows_launch(const MmArgs &a, const char *who)
+static int mm_rows_launch(const MmArgs &a, const char *who, int rm = 16, int rn = 16)
 {
-    const int64_t mt = ceil_div(a.M, 16 * MT), nt = ceil_div(a.N, 16 * NT);
+    const int64_t mt = ceil_div(a.M, rm * MT), nt = ceil_div(a.N, rn * NT);
     NB_REQUIRE(mt * nt < (1LL << 32) / (64 * W), "%s: too many tiles", who);
     mx_mm_rows_kernel<FP8, O, MT, NT, W><<<dim3((unsigned)(mt * nt)), dim3(64 * W), 0, a.st>>>(
-        (O *)a.C, a.A, a.As, a.B, a.Bs, a.M, a.N, a.steps, nt, a.whole);
+        (O *)a.C, a.A, a.As, a.B, a.Bs, a.M, a.N, a.steps, nt, a.whole, rm, rn);
     return check_launch(who);
 }
 
@@ -451,50 +468,68 @@ static int mm_rows_launch(const MmArgs &a, const char *who)
 //   4096 x 16384        702 / 275    902 / 373   961 / 517  1070 / 716
 //   4096 x 1024         165 /  64     77 /  34    63 /  37    72 /  48
 //   1024 x 1024         163 /  63     75 /  32    42 /  23    29 /  18
-//     64 x 8192                                   42 /  23    29 /  19    30 /  25    36 /  28
+//    256 x 1024                                   42 /  22    29 /  18    18 /  14    21 /  16    27 /  19
+//     64 x 1024                                   42 /  22    29 /  18    18 /  14    12 /   9     9 /   7
 //     16 x 32768                                  45 /  24    43 /  24    31 /  26    38 /  31    52 / -
-//      1 x 32768                                  45 /  24    42 /  23    28 /  24    33 /  28    34 / 32
-//      1 x 8192                                   41 /  22    29 /  18    16 /  13     9 /   8
+//      1 x 32768                                  45 /  24    42 /  23    28 /  24    30 /  28    33 / 32
+//      1 x 16384                                  42 /  22    29 /  19    17 /  16    18 /  17    19 / 17
+//      1 x 8192                                   41 /  22    29 /  18    16 /  13    11 /   8     9 / -
+// The last kind's time goes with the row pieces that its loads touch, (E4M3: 8, E2M1: 4) + 1 per row of A and 5 per row of B
+// in four steps; where its tiles do not give every CU one, they are made of fewer rows (8 or 4 of the 16) on the side
+// that costs least: 1001 x 10 x 16384 E4M3 13.3 us with whole tiles, 10.2 with 8 rows, 8.8 with 4; 16 x 1000 x 32768 E2M1
+// 19.5, 16.3 with 8 rows of B, 13.3 with 8 of each; more than 256 tiles lose again (4 and 8 rows: 21).
 struct MmCost {
     int rows, columns;
     bool one_per_cu;      // a CU holds one workgroup: what fills the card comes in whole rounds of 256
     double alone, full;
 };
-constexpr MmCost kMmCosts[2][7] = {
+constexpr MmCost kMmCosts[2][6] = {
     // E2M1 x E2M1
     {{256, 256, true, 0.97, 1.07}, {128, 128, false, 0.50, 0.364}, {64, 128, false, 0.34, 0.253}, {64, 64, false, 0.27, 0.173},
-     {16, 64, false, 0.20, 0.18}, {16, 32, false, 0.10, 0.10}, {16, 16, false, 0.055, 0.055}},
+     {16, 64, false, 0.20, 0.18}, {16, 32, false, 0.11, 0.105}},
     // E4M3 x E2M1
     {{256, 256, true, 2.55, 2.74}, {128, 128, false, 1.15, 0.88}, {64, 128, false, 0.62, 0.469}, {64, 64, false, 0.45, 0.261},
-     {16, 64, false, 0.25, 0.22}, {16, 32, false, 0.14, 0.13}, {16, 16, false, 0.07, 0.06}},
+     {16, 64, false, 0.25, 0.22}, {16, 32, false, 0.15, 0.14}},
 };
 
-static int mm_choice(const MmArgs &a, bool fp8)
+struct MmPlan {
+    int kind, rm, rn;     // rm, rn: rows of A and B in a tile of the last kind
+};
+static MmPlan mm_plan(const MmArgs &a, bool fp8)
 {
-    int best = 0;
-    double least = 0;
-    for (int v = 0; v < 7; v++) {
+    MmPlan plan{6, 16, 16};
+    const auto pieces = [&](int rm, int rn) {
+        return (fp8 ? 9 : 5) * (int)std::min<int64_t>(rm, a.M) + 5 * (int)std::min<int64_t>(rn, a.N);
+    };
+    const auto tiles = [&](int rm, int rn) { return (double)ceil_div(a.M, rm) * (double)ceil_div(a.N, rn); };
+    for (int rm = 16; rm >= 4; rm /= 2)
+        for (int rn = 16; rn >= 4; rn /= 2)
+            if (tiles(rm, rn) <= 256.0 && pieces(rm, rn) < pieces(plan.rm, plan.rn)) plan = {6, rm, rn};
+    const double touched = 0.00032 * pieces(plan.rm, plan.rn);
+    double least = std::max(0.02 + touched, (0.04 + touched) * (tiles(plan.rm, plan.rn) / 256.0));
+    for (int v = 0; v < 6; v++) {
         if (v < 4 && a.steps > 65536) continue;                  // longer rows than the tiles' offsets reach
         const MmCost &c = kMmCosts[fp8][v];
         double rounds = (double)ceil_div(a.M, c.rows) * (double)ceil_div(a.N, c.columns) / 256.0;
         if (c.one_per_cu) rounds = ceil(rounds);
         const double cost = std::max(c.alone, c.full * rounds);
-        if (least == 0 || cost < least) best = v, least = cost;
+        if (cost < least) plan.kind = v, least = cost;
     }
-    return best;
+    return plan;
 }
 
 template <bool FP8, typename O>
 static int mm_launch(const MmArgs &a, const char *who)
 {
-    switch (mm_choice(a, FP8)) {
+    const MmPlan plan = mm_plan(a, FP8);
+    switch (plan.kind) {
         case 0: return mm_tile_launch<FP8, O, 4, 2, 4, 8, FP8 ? 3 : 4>(a, who);
         case 1: return mm_tile_launch<FP8, O, 2, 2, 4, 4, 3>(a, who);
         case 2: return mm_tile_launch<FP8, O, 2, 2, 2, 4, 4>(a, who);
         case 3: return mm_tile_launch<FP8, O, 4, 1, 1, 4, 4>(a, who);
         case 4: return mm_rows_launch<FP8, O, 1, 4, 4>(a, who);
         case 5: return mm_rows_launch<FP8, O, 1, 2, 4>(a, who);
-        default: return mm_rows_launch<FP8, O, 1, 1, 8>(a, who);
+        default: return mm_rows_launch<FP8, O, 1, 1, 8>(a, who, plan.rm, plan.rn);
     }
 }
 

@@ -514,3 +514,27 @@ def test_captured_and_on_another_stream(ops):
         torch.cuda.synchronize()
         for a, b, c in zip(want, out, other):
             assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# products whose tiles are made of fewer rows so that every CU has one, whole chunks and odd steps, a row to every side
+FEW = [(1001, 10, 16000), (16, 1000, 2100), (15, 1001, 16384), (1, 1024, 512), (64, 500, 640), (1000, 1, 900), (5, 7, 50000),
+       (250, 13, 700), (120, 33, 1300), (600, 3, 128), (3, 2000, 129), (63, 65, 4096)]
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+@pytest.mark.parametrize("shape", FEW, ids=lambda s: "x".join(map(str, s)))
+def test_product_of_few_rows(ops, shape, a_format):
+    M, N, K = shape
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    a = torch.randn(M, K, generator=g, device="cuda") * torch.exp2(torch.randint(-6, 7, (M, 1), generator=g, device="cuda"))
+    b = torch.randn(N, K, generator=g, device="cuda") / 8
+    a[M // 2, K // 2] = float("nan")                         # one row of NaN, its neighbours none
+    A, B = ops.mx_quantize(a, a_format), ops.mx_quantize(b, "fp4")
+    a, b = ops.mx_dequantize(A, torch.float32).double(), ops.mx_dequantize(B, torch.float32).double()
+    got = ops.mx_mm_nt(A, B).double()
+    assert bool(got[M // 2].isnan().all())
+    rest = torch.arange(M, device="cuda") != M // 2
+    got, a = got[rest], a[rest]
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    adds = 2 * 17 * (O.padded(K) // 128) + 64                # as in test_product
+    assert got.numel() == 0 or float(((got - want).abs() - adds * 2.0 ** -23 * size).max()) <= 0
