@@ -8,7 +8,11 @@
 // Rows of at most 64 entries: a wave per row, ranks by comparing all pairs.  Up to 16384: a workgroup per row.  Longer
 // ones: one kernel over chunks of 8192 entries (the exponentials, which bound the whole, are then spread over the card
 // however few the rows), one workgroup per row to finish from the chunks' histograms.
-// Measured (MI355X, logits N(0, 2.5^2)): see the table in the launch function.
+//
+// What bounds it: rows of up to 16376 entries and few rows of any length, the latency of about ten phases that follow each
+// other (a phase 1 to 4 us, most of it waiting for one workgroup's instructions and for memory); 256 x 131072 bf16 with a
+// cut, 90 us: 48 us the exponentials' kernel (37 instructions an entry, two thirds of the cycles), 42 us the rows' kernel, 10
+// of them the second look at every logit at what the last cache gives to all CUs (7 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -50,23 +54,30 @@ struct TokenKey {
 #pragma unroll
         for (int e = 0; e < 8; e++) k[e] = token_key(v[e]);
     }
-    static __device__ __forceinline__ void value8(double (&d)[8], const T *p)
-    {
-        float v[8];
-        mx_load8(v, p);
-#pragma unroll
-        for (int e = 0; e < 8; e++) d[e] = (double)fmaxf(v[e], -__builtin_inff());       // NaN: -inf
-    }
+    typedef float Value;                                 // holds every logit, and -inf
+    static __device__ __forceinline__ void value8(float (&d)[8], const T *p) { mx_load8(d, p); }
     static __device__ __forceinline__ uint32_t key_of(double v) { return token_key((float)v); }
-    // logits as they compare cheapest; plain(k): the logit of a key, for windows of them (0 and what is above +inf's key: the
-    // ends of what can be drawn)
-    typedef float Plain;
-    static __device__ __forceinline__ void plain8(float (&v)[8], const T *p) { mx_load8(v, p); }
-    static __device__ __forceinline__ float plain(uint32_t k)
-    {
-        return k < 0x00800000u ? -3.402823466e38f : k > 0xFF800000u ? __builtin_inff()
-                                                                    : __builtin_bit_cast(float, k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu));
-    }
+    // Near: a window of keys as the cheapest test on logits as they lie in memory, at most a little wider: two operations an
+    // entry.  Differences are monotonic in v, so their roundings are too.
+    struct Near {
+        float middle, reach;
+        __device__ __forceinline__ Near(uint32_t from, uint32_t to)              // 0, and what is above +inf's key: no end
+        {
+            const float lo = from < 0x00800000u ? -3.402823466e38f : (float)value(from);
+            const float hi = to > 0xFF800000u ? __builtin_inff() : to < 0x00800000u ? -3.402823466e38f : (float)value(to);
+            const bool all = !(hi - lo < __builtin_inff());
+            middle = all ? 0.f : 0.5f * lo + 0.5f * hi;
+            reach = all ? __builtin_inff() : fmaxf(hi - middle, middle - lo);
+        }
+        __device__ __forceinline__ bool any(const T *p) const                    // of a group's entries; NaNs are not
+        {
+            float v[8], least = __builtin_inff();
+            mx_load8(v, p);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) least = fminf(fminf(least, fabsf(v[e] - middle)), fabsf(v[e + 1] - middle));
+            return least <= reach;
+        }
+    };
     // a key not above (not below) those of all logits of at least (at most) v, a few units of fp32 off
     static __device__ __forceinline__ uint32_t below(double v)
     {
@@ -92,19 +103,25 @@ struct TokenKey<int32_t> {
 #pragma unroll
         for (int e = 0; e < 8; e++) k[e] ^= 0x80000000u;
     }
+    typedef double Value;
     static __device__ __forceinline__ void value8(double (&d)[8], const int32_t *p)
     {
         const int4 a = reinterpret_cast<const int4 *>(p)[0], b = reinterpret_cast<const int4 *>(p)[1];
         d[0] = a.x, d[1] = a.y, d[2] = a.z, d[3] = a.w, d[4] = b.x, d[5] = b.y, d[6] = b.z, d[7] = b.w;
     }
     static __device__ __forceinline__ uint32_t key_of(double v) { return (uint32_t)(int32_t)v ^ 0x80000000u; }
-    typedef int32_t Plain;
-    static __device__ __forceinline__ void plain8(int32_t (&v)[8], const int32_t *p)
-    {
-        const int4 a = reinterpret_cast<const int4 *>(p)[0], b = reinterpret_cast<const int4 *>(p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-    static __device__ __forceinline__ int32_t plain(uint32_t k) { return (int32_t)(k ^ 0x80000000u); }
+    struct Near {
+        uint32_t from, span;
+        __device__ __forceinline__ Near(uint32_t from_, uint32_t to) : from(from_), span(to - from_) {}
+        __device__ __forceinline__ bool any(const int32_t *p) const
+        {
+            uint32_t k[8], least = 0xFFFFFFFFu;
+            key8(k, p);
+#pragma unroll
+            for (int e = 0; e < 8; e++) least = k[e] - from < least ? k[e] - from : least;
+            return least <= span;
+        }
+    };
     static __device__ __forceinline__ uint32_t below(double v)
     {
         if (!(v > -2147483640.0)) return 0u;
@@ -179,19 +196,20 @@ struct TokenLogits {
         return have;
     }
     // an edge group's logits, -inf for those that are not there or cannot be drawn
-    static __device__ __forceinline__ void edge_values(double (&d)[8], int j, const TokenEdges *edges)
+    static __device__ __forceinline__ void edge_values(typename TokenKey<T>::Value (&d)[8], int j, const TokenEdges *edges)
     {
         const int which = j ? 1 : 0;
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            d[e] = edges->have[which] >> e & 1 ? TokenKey<T>::value(edges->key[which][e]) : -__builtin_inf();
+            d[e] = (typename TokenKey<T>::Value)(edges->have[which] >> e & 1 ? TokenKey<T>::value(edges->key[which][e])
+                                                                             : -__builtin_inf());
     }
 };
 
-// 2^(u / 256) for u <= 0 as an integer multiple of 2^-frac, rounded (frac <= 51).  u = 256 n + j + r with |r| <= 1/2 and
-// 0 <= j < 256: 2^n by the exponent, 2^(j / 256) from a table, 2^(r / 256) by its Taylor sum to the fourth power, whose rest
-// is below 4e-17.  Adding 1.5 * 2^52 rounds u to an integer that then is the low word; adding 2^52 does the same for the
-// weight, whose bits below the exponent are the integer.  Fourteen 64-bit operations; the exponentials bound the long rows.
+// Weights.  With u = 256 times the octaves of a weight: u = 256 n + j + r, |r| <= 1/2 and 0 <= j < 256, and 2^(u / 256) is 2^n by
+// the exponent, 2^(j / 256) from a table, which also holds the weight of 1, 2^frac (frac <= 51), and 2^(r / 256) by its
+// Taylor sum to the fourth power, whose rest is below 4e-17.  Adding 1.5 * 2^52 rounds u to an integer that then is the low
+// word; adding 2^52 does the same for the weight, whose bits below the exponent are the integer.
 constexpr int kExpTable = 256;
 struct TokenExp {
     double power[kExpTable];                             // 2^(j / 256), j = 0 ... 255
@@ -209,50 +227,84 @@ constexpr TokenExp token_powers()
 }
 __device__ const TokenExp kTokenPowers = token_powers();
 // the table into LDS, by the whole workgroup; the caller's next barrier makes it visible
-__device__ __forceinline__ void token_exp_table(TokenExp *t)
+__device__ __forceinline__ void token_exp_table(TokenExp *t, int frac)
 {
-    for (int j = threadIdx.x; j < kExpTable; j += blockDim.x) t->power[j] = kTokenPowers.power[j];
+    const double one = (double)(1ull << frac);
+    for (int j = threadIdx.x; j < kExpTable; j += blockDim.x) t->power[j] = kTokenPowers.power[j] * one;
 }
-__device__ __forceinline__ uint64_t token_exp2(double u, int frac, const TokenExp *t)
+constexpr double kExpHalf = 6755399441055744.0;          // 1.5 * 2^52
+constexpr double kExpZero = -20000.0;                    // u from here on: 2^-78, 0 for every frac
+__device__ __forceinline__ int token_low(double y) { return (int)(uint32_t)__builtin_bit_cast(uint64_t, y); }
+struct TokenTaylor {
+    double c[5];
+    // of 2^((r - at) / 256)
+    __device__ __forceinline__ explicit TokenTaylor(double at = 0.0)
+    {
+        constexpr double a = 0.69314718055994530942 / kExpTable;
+        constexpr double k[5] = {1.0, a, a * a / 2, a * a * a / 6, a * a * a * a / 24};
+        const double f = fma(fma(fma(fma(k[4], -at, k[3]), -at, k[2]), -at, k[1]), -at, 1.0);
+#pragma unroll
+        for (int i = 0; i < 5; i++) c[i] = f * k[i];
+    }
+    // the weight of i + r, i = 256 n + j
+    __device__ __forceinline__ uint64_t weight(int i, double r, const TokenExp *t) const
+    {
+        const double p = fma(fma(fma(fma(c[4], r, c[3]), r, c[2]), r, c[1]), r, c[0]) * t->power[i & (kExpTable - 1)];
+        const uint64_t bits = __builtin_bit_cast(uint64_t, p);           // never near a subnormal: n >= -79
+        const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)(i & ~(kExpTable - 1)) << 12);
+        const double v = __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)bits) + 4503599627370496.0;
+        return __builtin_bit_cast(uint64_t, v) & 0xFFFFFFFFFFFFFull;
+    }
+};
+__device__ __forceinline__ uint64_t token_exp2(double u, const TokenExp *t)
 {
-    constexpr double a = 0.69314718055994530942 / kExpTable;
-    constexpr double c2 = a * a / 2, c3 = a * a * a / 6, c4 = a * a * a * a / 24;
-    constexpr double half = 6755399441055744.0;          // 1.5 * 2^52
-    u = fmax(u, -20000.0);                               // 2^-78: 0 for every frac
-    const double y = u + half;
-    const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, y);
-    const double r = u - (y - half);
-    const double p = fma(fma(fma(fma(c4, r, c3), r, c2), r, a), r, 1.0) * t->power[i & (kExpTable - 1)];
-    const double v = __builtin_amdgcn_ldexp(p, (i >> 8) + frac) + 4503599627370496.0;
-    return __builtin_bit_cast(uint64_t, v) & 0xFFFFFFFFFFFFFull;
+    u = fmax(u, kExpZero);
+    const double y = u + kExpHalf;
+    return TokenTaylor().weight(token_low(y), u - (y - kExpHalf), t);
 }
+
+// Bins.  A logit v lies at step rint(256 v * octaves per unit) of one grid for all chunks of a row, 32 steps to a bin: the same
+// for equal logits and rising with them.  Only the low words of steps are used: below the maximum by less than 20000
+// steps, or taken to lie there.  A maximum beyond 2^50 steps is alone: another fp32 value is 2^26 steps off, another int32 2^19,
+// and has no weight.
+constexpr int kStepsPerBin = kExpTable / kSlotsPerOctave;
+__device__ __forceinline__ bool token_alone(double vmax, double rate256) { return !(fabs(vmax) * rate256 < 0x1p50); }
 
 // How a row's logits become weights, relative to a maximum (the row's, or a chunk's)
 template <typename T>
 struct TokenScale {
     uint32_t kmax;
     double vmax, rate256;   // 256 times the octaves of the weight per unit of the logits
-    double per;             // bins per unit
-    int frac;
+    double low;             // what lies further below has no weight
+    int frac, last;         // last: the last step of the maximum's bin
+    bool alone;
     const TokenExp *table;
     __device__ __forceinline__ TokenScale(uint32_t kmax_, double rate, int frac_, const TokenExp *t)
-        : kmax(kmax_), vmax(TokenKey<T>::value(kmax_)), rate256(rate * kExpTable), per(rate * kSlotsPerOctave), frac(frac_), table(t) {}
+        : kmax(kmax_), vmax(TokenKey<T>::value(kmax_)), rate256(rate * kExpTable), low(vmax + kExpZero / rate256), frac(frac_),
+          last(token_low(fma(vmax, rate256, kExpHalf)) | (kStepsPerBin - 1)), alone(token_alone(vmax, rate256)), table(t) {}
     __device__ __forceinline__ uint64_t weight(uint32_t k) const
     {
-        const uint64_t w = token_exp2((TokenKey<T>::value(k) - vmax) * rate256, frac, table);
+        const uint64_t w = token_exp2((TokenKey<T>::value(k) - vmax) * rate256, table);
         return k == kmax ? 1ull << frac : w;             // also where both are +inf
     }
-    // Bins lie on one grid for all chunks of a row; they are the same for equal logits and rise with them.
-    static __device__ __forceinline__ double bin(uint32_t k, double rate)
-    {
-        return floor(TokenKey<T>::value(k) * (rate * kSlotsPerOctave));
-    }
-    // bins below the maximum's; the infinity's own bin is 0
-    __device__ __forceinline__ int slot(uint32_t k, double top) const
+    // bins below the maximum's
+    __device__ __forceinline__ int slot(uint32_t k) const
     {
         if (k == kmax) return 0;
-        const double d = top - floor(TokenKey<T>::value(k) * per);
-        return d < kSlots - 1 ? (int)d : kSlots - 1;
+        const uint32_t step = (uint32_t)token_low(fma(fmax(TokenKey<T>::value(k), low), rate256, kExpHalf));
+        const uint32_t d = ((uint32_t)last - step) / kStepsPerBin;
+        return alone || d >= kSlots ? kSlots - 1 : (int)d;
+    }
+    // keys that can lie in a slot, a little more than those that do: from ... to
+    __device__ __forceinline__ void window(int s, uint32_t &from, uint32_t &to) const
+    {
+        from = 0, to = kmax;
+        if (alone) return;
+        const double end = (fma(vmax, rate256, kExpHalf) - kExpHalf) + (double)(last & (kStepsPerBin - 1)) -
+                           (double)(token_low(fma(vmax, rate256, kExpHalf)) & (kStepsPerBin - 1)) - (double)(s * kStepsPerBin);
+        if (s < kSlots - 1) from = TokenKey<T>::below((end - kStepsPerBin + 0.5) / rate256);
+        const uint32_t above = s ? TokenKey<T>::above((end + 0.5) / rate256) : kmax;
+        to = above < kmax ? above : kmax;
     }
 };
 
@@ -314,7 +366,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void sample_short_kernel(TokenArgs a)
 {
     __shared__ TokenExp table;
-    token_exp_table(&table);
+    token_exp_table(&table, a.frac_bits);
     __syncthreads();
     const int lane = threadIdx.x & 63, V = a.V;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -370,17 +422,19 @@ struct TokenChunk {
 static_assert(sizeof(TokenChunk) % 16 == 0, "records of the workspace");
 
 // A workgroup takes chunk after chunk, the next one's loads under way while it works on one (a workgroup per chunk spent
-// most of its life waiting for them: 46 us instead of 33 for the exponentials of 256 x 131072).
+// most of its life waiting for them).  256 x 131072 bf16: 40 us, with the histogram 48, for the maximum alone 17.
+// Two workgroups a CU; three with 80 registers and spills 46 to 63, four 57 to 73.
 constexpr int kChunkGrid = 512;
 template <typename T>
-__global__ __launch_bounds__(512) void token_chunk_kernel(TokenArgs a)
+__global__ __launch_bounds__(512, 4) void token_chunk_kernel(TokenArgs a)
 {
+    typedef typename TokenKey<T>::Value Value;
     constexpr int WORDS = sizeof(T) / 2;                 // 16-byte words of a group
     __shared__ TokenExp table;
     __shared__ TokenEdges edges;
     __shared__ uint64_t hist_w[kSlots], sh_sum;
     __shared__ uint32_t hist_c[kSlots];
-    __shared__ double sh_max[2][8];
+    __shared__ Value sh_max[2][8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t items = (uint32_t)(a.R * a.chunks);
     uint4 next[2][WORDS];
@@ -401,7 +455,7 @@ __global__ __launch_bounds__(512) void token_chunk_kernel(TokenArgs a)
     };
     request(blockIdx.x);
     for (int t = tid; t < kSlots; t += 512) hist_w[t] = 0, hist_c[t] = 0;
-    token_exp_table(&table);
+    token_exp_table(&table, a.frac_bits);
     if (tid == 0) sh_sum = 0;
     int turn = 0;
     for (uint32_t item = blockIdx.x; item < items; item += gridDim.x, turn ^= 1) {
@@ -410,7 +464,7 @@ __global__ __launch_bounds__(512) void token_chunk_kernel(TokenArgs a)
         const TokenLogits<T> x(a.logits, row, a.V);
         const TokenSettings set(a, row);
         TokenChunk *out = reinterpret_cast<TokenChunk *>(a.workspace) + item;
-        double d[2][8];
+        Value d[2][8];
         bool whole[2];
 #pragma unroll
         for (int q = 0; q < 2; q++) {
@@ -428,47 +482,59 @@ __global__ __launch_bounds__(512) void token_chunk_kernel(TokenArgs a)
         for (int q = 0; q < 2; q++)
             if (!whole[q]) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) d[q][e] = -__builtin_inf();
+                for (int e = 0; e < 8; e++) d[q][e] = -(Value)__builtin_inf();
                 if (j0 + q * 512 < x.groups) x.edge_values(d[q], j0 + q * 512, &edges);
             }
-        double m = -__builtin_inf();
+        Value m = -(Value)__builtin_inf();
 #pragma unroll
-        for (int e = 0; e < 8; e++) m = fmax(m, fmax(d[0][e], d[1][e]));
+        for (int e = 0; e < 8; e++) m = fmax(m, fmax(d[0][e], d[1][e]));         // without NaNs
         m = wave_max(m);
         if (lane == 0) sh_max[turn][wave] = m;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < 8; w++) m = fmax(m, sh_max[turn][w]);
-        const bool any = m > -__builtin_inf();
+        const bool any = m > -(Value)__builtin_inf();
         if (any && !set.greedy) {
-            if (m == __builtin_inf()) {                  // the infinities share the weight; all others have none
+            double rate256 = set.rate * kExpTable, from = m;
+            if (token_alone(m, rate256)) {               // the maximum's likes share the weight, all others have none
 #pragma unroll
                 for (int q = 0; q < 2; q++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) d[q][e] = d[q][e] == m ? 0.0 : -__builtin_inf();
+                    for (int e = 0; e < 8; e++) d[q][e] = d[q][e] == m ? (Value)0 : -(Value)__builtin_inf();
+                from = 0.0, rate256 = 1.0;
             }
-            const double from = m == __builtin_inf() ? 0.0 : m, rate256 = set.rate * kExpTable;
-            const double per = set.rate * kSlotsPerOctave, top = floor(from * per);
+            const double low = from + kExpZero / rate256, y0 = fma(from, rate256, kExpHalf);
+            const int first = token_low(y0);
+            const uint32_t last = (uint32_t)first | (kStepsPerBin - 1);
+            const TokenTaylor taylor(fma(from, rate256, kExpHalf - y0));
             const bool cut = set.cut(), counted = set.top_k > 0;
             uint64_t sum = 0;
             // eight at a time: their chains of dependent operations run side by side
-            const auto take = [&](const double (&v)[8]) {
+            const auto take = [&](const Value (&v)[8]) {
+                int step[8];
                 uint64_t w[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) w[e] = token_exp2((v[e] - from) * rate256, a.frac_bits, &table);
+                for (int e = 0; e < 8; e++) {
+                    const double x = fmax((double)v[e], low), y = fma(x, rate256, kExpHalf);     // NaN: low
+                    step[e] = token_low(y);
+                    w[e] = taylor.weight((int)((uint32_t)step[e] - (uint32_t)first), fma(x, rate256, kExpHalf - y), &table);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; e++) sum += w[e];
                 if (cut) {
-                    int at[8];
+                    uint32_t at[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) at[e] = (int)fmin(top - floor(v[e] * per), (double)(kSlots - 1));
+                    for (int e = 0; e < 8; e++) {
+                        at[e] = (last - (uint32_t)step[e]) / kStepsPerBin;
+                        at[e] = at[e] < kSlots ? at[e] : kSlots - 1;
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; e++)
                         if (w[e]) atomicAdd((unsigned long long *)&hist_w[at[e]], (unsigned long long)w[e]);
                     if (counted) {
 #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            if (v[e] > -__builtin_inf()) atomicAdd(&hist_c[at[e]], 1u);
+                            if (v[e] > -(Value)__builtin_inf()) atomicAdd(&hist_c[at[e]], 1u);
                     }
                 }
             };
@@ -509,7 +575,8 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     constexpr uint32_t kList = LOCAL ? 1024 : kTokenList;
     __shared__ TokenExp table;
     __shared__ TokenEdges edges;
-    __shared__ uint64_t seg_w[SEGS];                     // what is kept of a segment; tie counts before
+    __shared__ uint64_t seg_w[SEGS];                     // what is kept of a segment; tie counts and indexes before
+    static_assert(LOCAL || sizeof(seg_w) >= kList * sizeof(uint32_t), "room for a list's indexes");
     __shared__ double slot_w[kSlots];
     __shared__ uint64_t hist_w[kSlots];                  // LOCAL: by slot; later by digit
     __shared__ uint32_t hist_c[kSlots], slot_c[kSlots];
@@ -517,13 +584,23 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     __shared__ double chunk_f[CHUNKS];
     __shared__ int chunk_off[CHUNKS];
     __shared__ uint64_t chunk_w[CHUNKS];                 // what is kept of a chunk
+    __shared__ uint32_t chunk_k[CHUNKS];                 // their largest keys
+    constexpr int PARTS = LOCAL ? 1 : THREADS / kSlots;
+    __shared__ double part_w[PARTS][kSlots];             // a row's histogram from every PARTS-th chunk
+    __shared__ uint32_t part_c[PARTS][kSlots];
     __shared__ uint32_t sh_key[WAVES], sh_have[WAVES], low_c[WAVES], sh_n, sh_count, sh_ties;
     __shared__ uint64_t sh_sum;
     __shared__ double low_w[WAVES], sh_before;
     __shared__ int sh_at;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
-    token_exp_table(&table);
+    // the chunks' heads, a thread each, under way from the start
+    static_assert(LOCAL || kTokenMaxChunks <= THREADS, "a thread per chunk");
+    const TokenChunk *chunk = reinterpret_cast<const TokenChunk *>(a.workspace) + row * a.chunks;
+    uint32_t head_max = 0, head_have = 0;
+    uint64_t head_sum = 0;
+    if (!LOCAL && tid < a.chunks) head_max = chunk[tid].kmax, head_have = chunk[tid].have, head_sum = chunk[tid].sum;
+    token_exp_table(&table, a.frac_bits);
     if (tid == 0) sh_at = a.V;
     if (LOCAL)
         for (int t = tid; t < kSlots; t += THREADS) hist_w[t] = 0, hist_c[t] = 0;
@@ -532,7 +609,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     __syncthreads();
     const TokenSettings set(a, row);
     const int segs = (x.groups + kSegGroups - 1) / kSegGroups;
-    const TokenChunk *chunk = reinterpret_cast<const TokenChunk *>(a.workspace) + row * a.chunks;
     uint32_t held[LOCAL ? HELD : 1][8], held_have[LOCAL ? HELD : 1];
     if constexpr (LOCAL) {
 #pragma unroll
@@ -579,8 +655,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
             for (int e = 0; e < 8; e++) m = k[e] > m ? k[e] : m;
         });
     } else {
-        for (int c = tid; c < a.chunks; c += THREADS)
-            if (chunk[c].have) any = 1, m = chunk[c].kmax > m ? chunk[c].kmax : m;
+        any = head_have, m = head_have ? head_max : 0u;
     }
     m = wave_max(m);
     any = __ballot(any) != 0;
@@ -595,8 +670,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     if (set.greedy) {
         int seg0 = 0, seg1 = segs;
         if constexpr (!LOCAL) {                          // the first chunk with that maximum
-            for (int c = tid; c < a.chunks; c += THREADS)
-                if (chunk[c].have && chunk[c].kmax == m) atomicMin(&sh_at, c);
+            if (head_have && head_max == m) atomicMin(&sh_at, tid);
             __syncthreads();
             seg0 = sh_at * (kChunkGroups / kSegGroups);
             seg1 = seg0 + kChunkGroups / kSegGroups < segs ? seg0 + kChunkGroups / kSegGroups : segs;
@@ -615,7 +689,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
         return;
     }
     const TokenScale<T> scale(m, set.rate, a.frac_bits, &table);
-    const double top = TokenScale<T>::bin(m, set.rate);
     // The smallest key that reaches min_p (weights rise with keys): 64 keys at a time, six bits of it per turn.
     uint32_t min_key = 0;
     if (set.min_p > 0.0) {
@@ -630,12 +703,11 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
         }
     }
     if constexpr (!LOCAL) {
-        for (int c = tid; c < a.chunks; c += THREADS) {
-            const uint32_t cm = chunk[c].kmax;
-            const double d = cm == m ? 0.0 : top - TokenScale<T>::bin(cm, set.rate);
-            chunk_off[c] = !chunk[c].have ? kSlots : d < kSlots - 1 ? (int)d : kSlots - 1;
-            chunk_f[c] = !chunk[c].have ? 0.0 : cm == m ? 1.0 : exp2((TokenKey<T>::value(cm) - scale.vmax) * set.rate);
-            chunk_w[c] = !chunk[c].have ? 0 : chunk[c].sum;
+        if (tid < a.chunks) {
+            chunk_k[tid] = head_max;
+            chunk_off[tid] = head_have ? scale.slot(head_max) : kSlots;
+            chunk_f[tid] = !head_have ? 0.0 : head_max == m ? 1.0 : exp2((TokenKey<T>::value(head_max) - scale.vmax) * set.rate);
+            chunk_w[tid] = head_have ? head_sum : 0;
         }
         __syncthreads();
     }
@@ -651,7 +723,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const uint64_t w = scale.weight(k[e]);
-                    const int s = scale.slot(k[e], top);
+                    const int s = scale.slot(k[e]);
                     if ((have >> e & 1) && w) atomicAdd((unsigned long long *)&hist_w[s], (unsigned long long)w);
                     if ((have >> e & 1) && set.top_k) atomicAdd(&hist_c[s], 1u);
                 }
@@ -659,39 +731,36 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
             __syncthreads();
             for (int t = tid; t < kSlots; t += THREADS) slot_w[t] = (double)hist_w[t], slot_c[t] = hist_c[t];
         } else {
-            // a chunk's bin s lies chunk_off bins lower in the row, its weights are chunk_f of the row's; chunk after chunk, so
-            // the sums have one order.  The last slot also takes all that lies below it (the other waves).
-            if (tid < kSlots - 1) {
-                double w = 0.0;
-                uint32_t n = 0;
-#pragma unroll 8
-                for (int c = 0; c < a.chunks; c++) {
-                    const int s = tid - chunk_off[c], at = s > 0 ? s : 0;        // no branch: the loads go out together
-                    const double f = s >= 0 ? chunk_f[c] : 0.0;
-                    w += f * (double)chunk[c].weight[at], n += s >= 0 ? chunk[c].count[at] : 0;
-                }
-                slot_w[tid] = w, slot_c[tid] = n;
-            } else if (wave >= kSlots / 64) {
-                constexpr int kWaves = WAVES - kSlots / 64 > 0 ? WAVES - kSlots / 64 : 1;
-                double w = 0.0;
-                uint32_t n = 0;
-                for (int c = wave - kSlots / 64; c < a.chunks; c += kWaves) {
-#pragma unroll
-                    for (int q = 0; q < kSlots / 64; q++) {
-                        const int s = q * 64 + lane;
-                        if (s + chunk_off[c] >= kSlots - 1 && chunk_off[c] < kSlots)
-                            w += chunk_f[c] * (double)chunk[c].weight[s], n += chunk[c].count[s];
-                    }
-                }
-                w = wave_sum(w), n = wave_sum(n);
-                if (lane == 0) low_w[wave] = w, low_c[wave] = n;
+            // a chunk's bin s lies chunk_off bins lower in the row, its weights are chunk_f of the row's; every PARTS-th chunk
+            // after the other, then the parts, so the sums have one order.  The last bin also takes all that lies below it.
+            const int part = tid / kSlots, mine = tid % kSlots;
+            double w = 0.0, low = 0.0;
+            uint32_t n = 0, low_n = 0;
+#pragma unroll 5
+            for (int c = part; c < a.chunks; c += PARTS) {
+                const int off = chunk_off[c], s = mine - off;
+                const bool below = off < kSlots && mine + off >= kSlots - 1;
+                uint64_t here_w = 0, below_w = 0;
+                uint32_t here_n = 0, below_n = 0;
+                if (s >= 0) here_w = chunk[c].weight[s], here_n = chunk[c].count[s];
+                if (below) below_w = chunk[c].weight[mine], below_n = chunk[c].count[mine];
+                w += chunk_f[c] * (double)here_w, n += here_n;
+                low += chunk_f[c] * (double)below_w, low_n += below_n;
             }
+            part_w[part][mine] = w, part_c[part][mine] = n;
+            low = wave_sum(low), low_n = wave_sum(low_n);
+            if (lane == 0) low_w[wave] = low, low_c[wave] = low_n;
             __syncthreads();
-            if (tid == 0) {
-                double w = 0.0;
-                uint32_t n = 0;
-                for (int v = kSlots / 64; v < WAVES; v++) w += low_w[v], n += low_c[v];
-                slot_w[kSlots - 1] = w, slot_c[kSlots - 1] = n;
+            if (tid < kSlots - 1) {
+                w = part_w[0][tid], n = part_c[0][tid];
+#pragma unroll
+                for (int q = 1; q < PARTS; q++) w += part_w[q][tid], n += part_c[q][tid];
+                slot_w[tid] = w, slot_c[tid] = n;
+            } else if (tid == kSlots - 1) {
+                w = 0.0, n = 0;
+#pragma unroll
+                for (int v = 0; v < WAVES; v++) w += low_w[v], n += low_c[v];
+                slot_w[tid] = w, slot_c[tid] = n;
             }
         }
         __syncthreads();
@@ -740,64 +809,71 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
             int slot = sh_at;
             uint32_t before_c = sh_count;
             double before_w = sh_before;
-            if (which == 2) slot = scale.slot(min_key, top);
+            if (which == 2) slot = scale.slot(min_key);
             if (slot < 0 || slot > border) continue;     // the row has no more than that: nothing is cut
             if (slot != border || !listed) {             // else the list of the border before is the one
                 // keys that can lie there, a little more than those that do
-                const uint32_t from = slot == kSlots - 1 ? 0u : TokenKey<T>::below((top - slot) / scale.per);
-                const uint32_t span = (slot == 0 ? 0xFFFFFFFFu : TokenKey<T>::above((top - slot + 1.0) / scale.per)) - from;
-                const typename TokenKey<T>::Plain lo = TokenKey<T>::plain(from), hi = TokenKey<T>::plain(from + span);
-                const auto put = [&](uint32_t k, int i) {
-                    if (scale.slot(k, top) == slot) {
+                uint32_t from, to;
+                scale.window(slot, from, to);
+                // the entries of a group that lie in the slot, into the list
+                const auto put = [&](const uint32_t (&keys)[8], uint32_t have, int i0) {
+                    uint32_t near = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) near |= (uint32_t)(keys[e] >= from && keys[e] <= to) << e;
+#pragma unroll 1
+                    for (near &= have; near; near &= near - 1) {
+                        const int e = __builtin_ctz(near);
+                        uint32_t k = keys[0];
+#pragma unroll
+                        for (int d = 1; d < 8; d++) k = d == e ? keys[d] : k;
+                        if (scale.slot(k) != slot) continue;
                         const uint32_t at = atomicAdd(&sh_n, 1u);
-                        if (at < kList) list[at] = TokenEntry{k, i};
+                        if (at < kList) list[at] = TokenEntry{k, i0 + e};
                     }
                 };
                 if constexpr (LOCAL) {
 #pragma unroll
-                    for (int q = 0; q < HELD; q++) {
-                        uint32_t near = 0;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) near |= (uint32_t)(held[q][e] - from <= span) << e;
-#pragma unroll 1
-                        for (near &= held_have[q]; near; near &= near - 1) {
-                            const int e = __builtin_ctz(near);
-                            uint32_t k = held[q][0];
-#pragma unroll
-                            for (int d = 1; d < 8; d++) k = d == e ? held[q][d] : k;
-                            put(k, (q * THREADS + tid) * kGroup - x.lead + e);
-                        }
-                    }
+                    for (int q = 0; q < HELD; q++) put(held[q], held_have[q], (q * THREADS + tid) * kGroup - x.lead);
                 } else {
-                    // one workgroup looks at the whole row: two comparisons an entry, on logits as they are
-                    constexpr int AHEAD = 4;
-                    if (tid < 2 * kGroup && (tid < kGroup ? !x.whole(0) : x.groups > 1 && !x.whole(x.groups - 1))) {
-                        const int which = tid / kGroup, e = tid % kGroup;
-                        const uint32_t k = edges.key[which][e];
-                        if ((edges.have[which] >> e & 1) && k - from <= span)
-                            put(k, (which ? x.groups - 1 : 0) * kGroup - x.lead + e);
-                    }
+                    // One workgroup looks at the whole row, which its instructions bound: first for the groups that have such an
+                    // entry, then, a thread each, for the entries.  (Entry by entry at once, a wave goes through all of that
+                    // for the few of its lanes that have one: 17 us more for 131072 entries.)
+                    constexpr int WORDS = sizeof(T) / 2, AHEAD = 8 / WORDS;      // 16-byte words of a group
+                    uint32_t *const found = reinterpret_cast<uint32_t *>(seg_w);
+                    const typename TokenKey<T>::Near near(from, to);
 #pragma unroll 1
                     for (int s = wave; s < segs; s += AHEAD * WAVES) {
-                        typename TokenKey<T>::Plain v[AHEAD][8];
-                        bool have[AHEAD];
+                        uint4 raw[AHEAD][WORDS];
 #pragma unroll
                         for (int q = 0; q < AHEAD; q++) {
                             const int j = (s + q * WAVES) * kSegGroups + lane;
-                            have[q] = s + q * WAVES < segs && x.whole(j);
-                            if (have[q]) TokenKey<T>::plain8(v[q], x.row + (j * kGroup - x.lead));
+                            if (x.whole(j)) {
+#pragma unroll
+                                for (int w = 0; w < WORDS; w++)
+                                    raw[q][w] = reinterpret_cast<const uint4 *>(x.row + (j * kGroup - x.lead))[w];
+                            }
                         }
 #pragma unroll
                         for (int q = 0; q < AHEAD; q++) {
-                            if (!have[q]) continue;
-                            uint32_t near = 0;
-#pragma unroll
-                            for (int e = 0; e < 8; e++) near |= v[q][e] >= lo && v[q][e] <= hi ? 1u << e : 0u;
-#pragma unroll 1
-                            for (; near; near &= near - 1) {
-                                const int i = ((s + q * WAVES) * kSegGroups + lane) * kGroup - x.lead + __builtin_ctz(near);
-                                put(TokenKey<T>::key1(x.row + i), i);    // again from memory: few of them
+                            const int j = (s + q * WAVES) * kSegGroups + lane;
+                            if (j < x.groups && (!x.whole(j) || near.any(reinterpret_cast<const T *>(raw[q])))) {
+                                const uint32_t at = atomicAdd(&sh_n, 1u);
+                                if (at < kList) found[at] = j;
                             }
+                        }
+                    }
+                    __syncthreads();
+                    const uint32_t n = sh_n;
+                    __syncthreads();
+                    if (n <= kList) {                    // else it stays: too many for the list
+                        if (tid == 0) sh_n = 0;
+                        __syncthreads();
+#pragma unroll 1
+                        for (uint32_t i = tid; i < n; i += THREADS) {
+                            uint32_t k[8];
+                            const int j = (int)found[i];
+                            const uint32_t have = x.load(k, j);
+                            put(k, have, j * kGroup - x.lead);
                         }
                     }
                 }
@@ -876,13 +952,13 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                                 uint32_t k = held[q][0];
 #pragma unroll
                                 for (int d = 1; d < 8; d++) k = d == __builtin_ctz(left) ? held[q][d] : k;
-                                if (scale.slot(k, top) == slot) put(k);
+                                if (scale.slot(k) == slot) put(k);
                             }
                     } else {
 #pragma unroll 1
                         for (int i = tid; i < a.V; i += THREADS) {
                             const uint32_t q = TokenKey<T>::key1(x.row + i);
-                            if (TokenKey<T>::drawable(q) && scale.slot(q, top) == slot) put(q);
+                            if (TokenKey<T>::drawable(q) && scale.slot(q) == slot) put(q);
                         }
                     }
                     __syncthreads();
@@ -947,7 +1023,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     if (!LOCAL && listed && ties < equal && key >= lowest) {
         // all entries equal to `key` are in the list: the one with ties - 1 of them before it
         uint32_t *const same = reinterpret_cast<uint32_t *>(seg_w);
-        static_assert(LOCAL || sizeof(seg_w) >= kList * sizeof(uint32_t), "room for their indexes");
         __syncthreads();
         if (tid == 0) sh_n = 0;
         __syncthreads();
@@ -1034,7 +1109,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                 const TokenEntry q = list[i];
                 if (!passes(q.key, q.index)) continue;
                 const int c = (q.index + x.lead) / (kGroup * kChunkGroups);
-                const TokenScale<T> sc(chunk[c].kmax, set.rate, a.frac_bits, &table);
+                const TokenScale<T> sc(chunk_k[c], set.rate, a.frac_bits, &table);
                 atomicAdd((unsigned long long *)&chunk_w[c], (unsigned long long)sc.weight(q.key));
             }
         }
@@ -1066,7 +1141,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
             constexpr int kSegsPerChunk = kChunkGroups / kSegGroups;
             seg0 = sh_at * kSegsPerChunk;
             seg1 = seg0 + kSegsPerChunk < segs ? seg0 + kSegsPerChunk : segs;
-            drawn_max = chunk[sh_at].kmax;
+            drawn_max = chunk_k[sh_at];
         }
     }
     const TokenScale<T> drawn(drawn_max, set.rate, a.frac_bits, &table);
@@ -1133,6 +1208,13 @@ static int token_chunks(int64_t V) { return (int)ceil_div(V + kGroup - 1, kChunk
 template <typename T>
 static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
 {
+    // Borders, in microseconds without a cut / with top_p = 0.9, logits N(0, 2.5^2), this kernel and the one for longer rows:
+    //   4096 x 64 fp32        9 /  15      23 /  46
+    //   1024 x 2000 bf16     10 /  21      26 /  65
+    //    256 x 8000 bf16      9 /  26      16 /  35 (by chunks)
+    //    256 x 16000 bf16    13 /  28      18 /  37 (by chunks)
+    //   1024 x 16000 fp32    52 / 111      69 / 134 (by chunks)
+    // By chunks: 64 x 32768 bf16 17 / 32, 1 x 131072 bf16 16 / 38, 256 x 131072 bf16 51 / 90, the largest entry alone 20.
     if (a.V <= 64)
         sample_short_kernel<T><<<dim3((unsigned)ceil_div(a.R, 4)), dim3(256), 0, st>>>(a);
     else if (a.V <= 256 * kGroup - 8)                    // a row that starts inside a group reaches into one more
