@@ -16,6 +16,7 @@ Additions that the reference lacks are grouped at the end (supplied-word / Philo
 sample+popcount product with a flip base, the fused conv->threshold->pack(->pool) op; the real-valued end of a network:
 microscaled 4- and 8-bit rows, the norm that writes them, their product, and tokens drawn from logits).
 """
+import ctypes
 import math
 
 import torch
@@ -1460,7 +1461,7 @@ def _row_setting(value, name, dtype, R, device):
         if value.device != device:
             raise RuntimeError("Tensors are on different devices")
         return value.data_ptr(), 0
-    value = int(value) if dtype == torch.int32 else float(value)
+    value = int(value) if dtype == torch.int32 else ctypes.c_float(value).value
     if value != value:
         raise ValueError("%s is NaN" % name)
     return None, value
@@ -1477,7 +1478,8 @@ def sample_tokens_from_words(logits, words, temperature=1.0, top_k=0, top_p=1.0,
     word / 2**32 of all kept ones.  ``temperature`` <= 0 takes the largest entry, the first of equal ones.
 
     ``words`` [R]: uint32 (or int32 holding the same bit patterns), e.g. from :func:`philox_words`.  Every setting is a
-    number for all rows or a tensor [R] (float32; ``top_k`` int32).  Weights are summed as integers: the same tokens
+    number for all rows or a tensor [R] (float32; ``top_k`` int32); numbers are rounded to float32 too, so that both draw the
+    same tokens.  Weights are summed as integers: the same tokens
     on every run.  Stands beside :func:`sample_bits_from_words`, which draws bits."""
     _check(logits, "logits")
     _check(words, "words")

@@ -99,7 +99,8 @@ def sample(logits, word, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One row (float64 logits) -> token.  Weights are whole multiples of 2^-f, as the format of the operator says: f =
     min(51, 61 - ceil(log2 V)) fraction bits; those below half a unit are 0.  (All of a row's zeros together stand for less
     than V 2^-(f+1) of the largest weight: 2^-28 at V = 131072 and at V <= 2^14 less than 2^-32, which only a word of 0 could
-    ask for.)"""
+    ask for.)  Settings are float32, as a tensor of them is."""
+    temperature, top_p, min_p = (float(np.float32(v)) for v in (temperature, top_p, min_p))
     x = [float(v) for v in logits]
     live = [i for i, v in enumerate(x) if v == v and v != -math.inf]
     if not live:

@@ -538,3 +538,14 @@ def test_product_of_few_rows(ops, shape, a_format):
     want, size = a @ b.t(), a.abs() @ b.abs().t()
     adds = 2 * 17 * (O.padded(K) // 128) + 64                # as in test_product
     assert got.numel() == 0 or float(((got - want).abs() - adds * 2.0 ** -23 * size).max()) <= 0
+
+
+def test_tokens_number_and_tensor_settings_are_one(ops):
+    # 10 equal entries, top_p the decimal 0.3: as float32 it is above 3/10, so a fourth entry is kept, and likewise 0.7 is below
+    R = 64
+    x = torch.zeros(R, 10, device="cuda")
+    words = words_of(R, 11).cuda()
+    for value, kept in ((0.3, 4), (0.7, 7), (0.1, 2), (0.9, 9)):
+        a = ops.sample_tokens_from_words(x, words, top_p=value)
+        b = ops.sample_tokens_from_words(x, words, top_p=torch.full((R,), value, device="cuda"))
+        assert torch.equal(a, b) and int(a.max()) == kept - 1
