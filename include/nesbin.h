@@ -559,7 +559,8 @@ int nb_mx_mm_nt(void *C, int type, const uint8_t *A, const uint8_t *A_scales, in
  * weights kept at indices up to i add up to more than words[r] / 2^32 of all that are kept.  T <= 0: the largest
  * entry, the first of equal ones.  A row in which nothing can be drawn gives -1.  A row's largest entry +inf: the
  * infinities share the weight equally.
- * Weights are held as integers (61 - ceil(log2 V) fraction bits, 51 at most), so sums do not depend on an order;
+ * Weights are held as integers (61 - ceil(log2 V) fraction bits, 51 at most, of the row's largest; in rows of more than
+ * 16376 entries of the largest of about 8192 neighbours, so some are finer), so sums do not depend on an order of work;
  * weights below half a unit of that are never drawn.
  * temperature, top_k, top_p, min_p: per-row arrays [R], or NULL for the value that follows each of them for all rows
  * (not NaN).  1 <= V <= 2^20.  workspace: nb_sample_tokens_workspace_bytes(R, V) bytes, 16-byte aligned (NULL if 0).

@@ -135,3 +135,13 @@ def sample(logits, word, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if acc > bar:
             return i
     raise AssertionError("unreachable: the word is below 2**32")
+
+
+def token_within(logits, word, token, slack, temperature=1.0):
+    """Whether a row's token, nothing cut off, is the drawn one with real weights and borders moved by up to ``slack`` of the
+    largest weight."""
+    x = np.asarray(logits, dtype=np.float64)
+    temperature = float(np.float32(temperature))
+    w = np.where(x == x.max(), 1.0, np.exp((x - x.max()) / temperature))
+    before, after, total = math.fsum(w[:token]), math.fsum(w[:token + 1]), math.fsum(w)
+    return w[token] > 0 and before - slack <= int(word) / 2 ** 32 * total <= after + slack

@@ -549,3 +549,158 @@ def test_tokens_number_and_tensor_settings_are_one(ops):
         a = ops.sample_tokens_from_words(x, words, top_p=value)
         b = ops.sample_tokens_from_words(x, words, top_p=torch.full((R,), value, device="cuda"))
         assert torch.equal(a, b) and int(a.max()) == kept - 1
+
+
+# ---- rows, starts and sizes that the tests above leave out ---------------------------------------------------------------
+HARD = [dict(), dict(top_p=0.9), dict(top_k=2500), dict(min_p=0.02), dict(top_k=100, top_p=0.5, min_p=0.3),
+        dict(temperature=1e-4, top_p=0.7), dict(temperature=1e4, top_p=0.7, min_p=0.99), dict(temperature=1e-12, top_p=0.9, top_k=3)]
+
+
+def hard_rows(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    whole = dtype == torch.int32
+    lowest = -2.0 ** 31 if whole else float(torch.finfo(dtype).min)
+    x = torch.zeros(8, V, dtype=torch.float64)
+    x[0] = lowest if whole else -float("inf")
+    x[0, [0, 5, V // 2, V - 9, V - 1]] = torch.tensor([1.0, -2.0, 0.5, 3.0, 2.0], dtype=torch.float64)
+    x[1, V // 3] = 30.0
+    x[2] = torch.randn(V, generator=g) * (1 if whole else 1e-4)
+    x[3] = torch.rand(V, generator=g) * (3 if whole else 0.05)               # thousands of entries in one bin
+    x[4] = torch.randn(V, generator=g) * (1e8 if whole else 1e4)
+    x[5] = torch.where(torch.rand(V, generator=g) < 0.9, lowest, torch.randn(V, generator=g).double() * 2)
+    x[6] = -7.0
+    x[7] = torch.linspace(-20, 0, V)
+    return (x.round() if whole else x).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int32], ids=IDS + ["i32"])
+@pytest.mark.parametrize("V", [777, 9001, 20011])
+def test_tokens_of_hard_rows(ops, V, dtype):
+    x = hard_rows(V, dtype)
+    for n, kw in enumerate(HARD):
+        words = words_of(8, n + 40)
+        if V < 16384 or n:
+            check_tokens(ops, x, words, **kw)
+            continue
+        # Rows in pieces take a piece's weights as multiples of 2^-f of the piece's largest, so some are finer than the oracle's
+        # multiples of 2^-f of the row's.  Either is off by at most 2^-(f + 1) of the row's largest: a running sum by
+        # V 2^-(f + 1), and the total times the word's fraction by as much again (f = 61 - 15 = 46 here).
+        got = ops.sample_tokens_from_words(x.cuda(), words.cuda(), **kw).cpu().tolist()
+        for r in range(8):
+            word = int(words[r]) & 0xFFFFFFFF
+            assert got[r] == O.sample(host(x)[r], word, **kw) or \
+                O.token_within(host(x)[r], word, got[r], 2 * V * 2.0 ** -47, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int32], ids=IDS + ["i32"])
+def test_tokens_from_any_start(ops, dtype):
+    """Rows that begin and end inside the 16 bytes of a load, with entries around them that would win."""
+    g = torch.Generator().manual_seed(9)
+    for V in (10, 501, 4999, 20003):
+        for start in (1, 3):
+            flat = torch.full((3 * V + 16,), 60000.0).to(dtype)
+            x = (torch.randn(3, V, generator=g) * (40 if dtype == torch.int32 else 2)).to(dtype)
+            flat[start:start + 3 * V] = x.view(-1)
+            there = flat.cuda()[start:start + 3 * V].view(3, V)
+            for n, kw in enumerate((dict(top_p=0.9, temperature=2.0), dict(temperature=0.0))):
+                w = words_of(3, n)
+                got = ops.sample_tokens_from_words(there, w.cuda(), **kw).cpu().tolist()
+                assert got == [O.sample(host(x)[r], int(w[r]) & 0xFFFFFFFF, **kw) for r in range(3)]
+
+
+@pytest.mark.parametrize("K", [65, 1500, 3001, 6007, 20001])
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int32], ids=IDS + ["i32"])
+def test_rows_from_any_start(ops, dtype, K):
+    """The conversions and the norm on tensors one element off a 16-byte border equal those on aligned copies."""
+    g = torch.Generator().manual_seed(K)
+    off = lambda t: torch.cat([t.new_full((1,), 50.0), t.reshape(-1)])[1:].view(t.shape)
+    x = (torch.randn(7, K, generator=g) * (30 if dtype == torch.int32 else 1)).to(dtype).cuda()
+    rdt = torch.float16 if dtype == torch.int32 else dtype
+    r, w = (torch.randn(n, generator=g).to(rdt).cuda() for n in ((7, K), (K,)))
+    assert off(x).data_ptr() % 16 and off(x).is_contiguous()
+    for format in O.FORMATS:
+        for res in (None, r):
+            a, ra = ops.rms_norm_mx(x, w, res, 1e-5, format)
+            b, rb = ops.rms_norm_mx(off(x), off(w), None if res is None else off(res), 1e-5, format)
+            assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+            assert res is None or torch.equal(ra, rb)
+            y, want = O.rms_norm(host(x), host(w), None if res is None else host(res), 1e-5,
+                                 (lambda v: v) if res is None else _rounder(rdt))
+            codes, scales = O.quantize(y.astype(np.float64), format)
+            assert np.array_equal(a.codes.cpu().numpy(), codes) and np.array_equal(a.scales.cpu().numpy(), scales)
+        if dtype != torch.int32:
+            a, b = ops.mx_quantize(x, format), ops.mx_quantize(off(x), format)
+            assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+@pytest.mark.parametrize("K", [500, 3000, 8000, 20000])
+def test_norm_with_the_residual_in_place(ops, K):
+    from nesgpu_amd import _lib
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x, r = (torch.randn(9, K, generator=g, device="cuda").bfloat16() for _ in range(2))
+    w = torch.ones(K, device="cuda")
+    want, new = ops.rms_norm_mx(x, w, r, 1e-5, "fp8")
+    codes, scales = torch.empty_like(want.codes), torch.empty_like(want.scales)
+    _lib.call("nb_rms_norm_mx", codes.data_ptr(), scales.data_ptr(), r.data_ptr(), x.data_ptr(), 2, r.data_ptr(), 2,
+              w.data_ptr(), 0, 1e-5, 1, 9, K, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(r, new) and torch.equal(codes, want.codes) and torch.equal(scales, want.scales)
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+@pytest.mark.parametrize("shape", [(3, 70, 1024), (300, 200, 1024), (1, 2000, 4096), (600, 700, 640)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_product_with_scales_on_four_bytes(ops, shape, a_format):
+    M, N, K = shape
+    g = torch.Generator(device="cuda").manual_seed(K)
+    A = ops.mx_quantize(torch.randn(M, K, generator=g, device="cuda"), a_format)
+    B = ops.mx_quantize(torch.randn(N, K, generator=g, device="cuda"), "fp4")
+
+    def moved(q, format):
+        flat = torch.zeros(q.scales.numel() + 16, dtype=torch.uint8, device="cuda")
+        flat[4:4 + q.scales.numel()] = q.scales.view(-1)
+        return ops.MXRows(q.codes, flat[4:4 + q.scales.numel()].view(q.scales.shape), K, format)
+
+    want = ops.mx_mm_nt(A, B)
+    for a, b in ((moved(A, a_format), B), (A, moved(B, "fp4")), (moved(A, a_format), moved(B, "fp4"))):
+        assert torch.equal(ops.mx_mm_nt(a, b), want)
+
+
+def test_rows_are_copied_and_pickled(ops):
+    import copy
+    import pickle
+    x = torch.randn(5, 200, device="cuda")
+    for q in (ops.mx_quantize(x), ops.mx_quantize(x, "fp8")):
+        want = ops.mx_dequantize(q)
+        for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+            assert torch.equal(ops.mx_dequantize(other), want)
+            q.codes, other.scales                                # parts made in one and not in the other
+            assert torch.equal(ops.mx_dequantize(other), want) and torch.equal(other.codes, q.codes)
+
+
+def test_offsets_past_32_bits(ops):
+    """The last rows of tensors of more than 2^31 elements (and bytes of codes) equal those rows alone."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows, K = 70001, 32768
+    tail = torch.randn(3, K, generator=g, device="cuda").bfloat16()
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = tail
+    one = ops.mx_quantize(tail, "fp8")
+    q = ops.mx_quantize(x, "fp8")
+    assert torch.equal(q.codes[-3:], one.codes) and torch.equal(q.scales[-3:], one.scales)
+    assert not bool(q.codes[:-3].any())
+    assert torch.equal(ops.mx_dequantize(q)[-3:], ops.mx_dequantize(one))
+    w = torch.ones(K, device="cuda")
+    n, new = ops.rms_norm_mx(x, w, x)
+    n1, new1 = ops.rms_norm_mx(tail, w, tail)
+    assert torch.equal(n.codes[-3:], n1.codes) and torch.equal(n.scales[-3:], n1.scales) and torch.equal(new[-3:], new1)
+    for N in (8, 300):
+        B = ops.mx_quantize(torch.randn(N, K, generator=g, device="cuda"), "fp4")
+        c, c1 = ops.mx_mm_nt(q, B)[-3:].double(), ops.mx_mm_nt(one, B).double()
+        size = ops.mx_dequantize(one, torch.float32).double().abs() @ ops.mx_dequantize(B, torch.float32).double().abs().t()
+        adds = 2 * 17 * (K // 128) + 64                      # as in test_product, for each of the two
+        assert float(((c - c1).abs() - 2 * adds * 2.0 ** -23 * size).max()) <= 0
+    del n, new, q
+    words = torch.randint(-2 ** 31, 2 ** 31, (rows,), generator=g, device="cuda").int()
+    for kw in (dict(top_p=0.9), dict(temperature=0.0)):
+        assert torch.equal(ops.sample_tokens_from_words(x, words, **kw)[-3:],
+                           ops.sample_tokens_from_words(tail, words[-3:].contiguous(), **kw))
