@@ -174,12 +174,20 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
 }
 
 // ---- tiles staged through LDS ----------------------------------------------------------------------------------------
-// A workgroup of WM x WN waves makes a tile of 16 MT WM x 16 NT WN outputs.  A step of 128 positions of its rows goes from
-// memory to LDS without passing registers (16 bytes per lane), two steps ahead of the products: three buffers, one
-// barrier per step.  LDS rows are as dense as in memory (64 bytes of E2M1, 128 of E4M3, which is what such a
+// A workgroup of WM x WN waves makes a tile of 16 MT WM x 16 NT WN outputs.  Its rows go from memory to LDS without passing
+// registers (16 bytes per lane), in stages of S steps of 128 positions, BUFFERS - 1 of them ahead of the products; one
+// barrier per stage.  LDS rows are as dense as in memory (64 bytes of E2M1 a step, 128 of E4M3, which is what such a
 // load writes); the 16-byte pieces of a row are permuted by the row's number, at the source address and again where
 // fragments are read, so that the 16 rows of a fragment read lie in different banks.  Scales come four steps at a time,
 // 16 bytes per row.
+//
+// What bounds it.  E2M1: the way from the second cache into LDS.  A tile of 256 x 256 takes 32 KB a step, of 128 x 128 16 KB,
+// and either arrives at 15 to 16 bytes a cycle and CU, however many stages are ahead (2, 3, 4 of 16 KB and 32 KB alike) and
+// however many CUs are at work (64, 256): 1.0 and 0.5 us a step, where the matrix instructions alone would take 0.45 and
+// 0.11.  8192 x 8192 x 8192 4.0 PFLOP/s.  E4M3: the matrix instructions, of which the split makes two, at 65 % of their rate.
+// Two steps a stage (128 bytes of every row, one stage ahead) are 2 to 5 % faster for 256 x 256 of E2M1: on random rows
+// 4096 x 16384 x 8192 306 us, 316 with one, 4096 x 8192 x 2048 52, 54.6; for the smaller tiles, whose waves have nobody to
+// take turns with, 10 to 20 % slower.
 template <int BYTES>
 __device__ __forceinline__ int mx_swizzle(int row)
 {
@@ -210,39 +218,39 @@ __device__ __forceinline__ void mx_wait_loads()
 
 __device__ __forceinline__ void mx_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-template <bool FP8, int WM, int WN, int MT, int NT, int BUFFERS>
+template <bool FP8, int WM, int WN, int MT, int NT, int S, int BUFFERS>
 struct MxTile {
+    static_assert(S == 1 || (S == 2 && !FP8), "a stage's row is 64 or 128 bytes");
     static constexpr int WAVES = WM * WN, TM = 16 * MT * WM, TN = 16 * NT * WN;
-    static constexpr int ABYTES = FP8 ? 128 : 64;
-    static constexpr int kStage = TM * ABYTES + TN * 64, kBuffers = BUFFERS, kAhead = BUFFERS - 1;   // stages ahead
+    static constexpr int ABYTES = FP8 ? 128 : 64, AROW = S * ABYTES, BROW = S * 64;   // a row's bytes of a step, of a stage
+    static constexpr int kStage = TM * AROW + TN * BROW, kBuffers = BUFFERS, kAhead = BUFFERS - 1;   // stages ahead
     static constexpr int kScales = (TM + TN) * 16;                       // four steps
     static constexpr int kLds = kBuffers * kStage + 2 * kScales;
     // A stage comes in 1 KB pieces (a wave's 64 lanes of 16 bytes), the scales in pieces of 64 rows.  Every wave asks for
     // the same number of them, so that its count of loads is known; where there are fewer pieces than that, some waves
     // ask for the first ones again.
-    static constexpr int A_PIECES = TM * ABYTES / 1024, B_PIECES = TN * 64 / 1024, S_PIECES = (TM + TN) / 64;
+    static constexpr int A_PIECES = TM * AROW / 1024, B_PIECES = TN * BROW / 1024, S_PIECES = (TM + TN) / 64;
     static constexpr int A_LOADS = (A_PIECES + WAVES - 1) / WAVES, B_LOADS = (B_PIECES + WAVES - 1) / WAVES;
     static constexpr int S_LOADS = (S_PIECES + WAVES - 1) / WAVES;
     static constexpr int LOADS = A_LOADS + B_LOADS;
-    // All but so many loads have arrived when stage s + 1 has, behind the loads of step s (the next group's scales and
-    // stage s + kAhead).  Where the scales lie among the later loads they are allowed for only if that is the newest stage:
-    // for more stages ahead the wait is then S_LOADS loads stricter than it need be, once in four steps.
+    // All but so many loads have arrived when the next stage has, behind those that a stage's first step asked for (the next
+    // group's scales, where it begins a group of four steps, then the stage kAhead further).  With two stages ahead the
+    // scales lie among the allowed ones; with more the wait is S_LOADS loads stricter than it need be once in a group.
     static constexpr int wait(bool group) { return (kAhead - 1) * LOADS + (kAhead == 2 && group ? S_LOADS : 0); }
-    // the waits below: a group of scales, asked for four steps before its first use, has arrived with all but the latest
-    // kAhead - 1 stages
-    static_assert(kAhead >= 2 && kAhead <= 5, "stages ahead");
+    // a group of scales, asked for four steps before its first use, has arrived with all but the latest kAhead - 1 stages
+    static_assert(kAhead >= 1 && kAhead <= 4 / S + 1, "stages ahead");
     static_assert(TM % 64 == 0 && TN % 64 == 0 && kLds <= 160 * 1024, "LDS");
     static constexpr int64_t kMaxSteps = (1LL << 31) / (TM > TN ? TM : TN) / ABYTES - 1;   // 32-bit offsets
 };
 
-template <bool FP8, typename O, int WM, int WN, int MT, int NT, int BUFFERS>
+template <bool FP8, typename O, int WM, int WN, int MT, int NT, int S, int BUFFERS>
 __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict__ C, const uint8_t *__restrict__ A,
                                                                   const uint32_t *__restrict__ As,
                                                                   const uint8_t *__restrict__ B,
                                                                   const uint32_t *__restrict__ Bs, int M, int N,
                                                                   int steps, int mtiles, int ntiles, bool whole)
 {
-    using P = MxTile<FP8, WM, WN, MT, NT, BUFFERS>;
+    using P = MxTile<FP8, WM, WN, MT, NT, S, BUFFERS>;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
@@ -262,17 +270,22 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
     const uint8_t *const a_tile = A + (int64_t)m0 * steps * P::ABYTES, *const b_tile = B + (int64_t)n0 * steps * 64;
     const int a_last = M - 1 - m0, b_last = N - 1 - n0;
     uint32_t a_src[P::A_LOADS], b_src[P::B_LOADS], s_src[P::S_LOADS];
+    uint32_t a_step[P::A_LOADS], b_step[P::B_LOADS];                     // bytes into the stage's later steps
 #pragma unroll
     for (int q = 0; q < P::A_LOADS; q++) {
-        constexpr int lanes = P::ABYTES / 16;                            // lanes per row
+        constexpr int lanes = P::AROW / 16;                              // lanes per row
         const int row = (q * P::WAVES + wave) % P::A_PIECES * (64 / lanes) + lane / lanes;
-        a_src[q] = (uint32_t)((row < a_last ? row : a_last) * steps * P::ABYTES +
-                              16 * ((lane % lanes) ^ mx_swizzle<P::ABYTES>(row)));
+        const int at = 16 * ((lane % lanes) ^ mx_swizzle<P::AROW>(row));
+        a_src[q] = (uint32_t)((row < a_last ? row : a_last) * steps * P::ABYTES + at);
+        a_step[q] = at / P::ABYTES * P::ABYTES;
     }
 #pragma unroll
     for (int q = 0; q < P::B_LOADS; q++) {
-        const int row = (q * P::WAVES + wave) % P::B_PIECES * 16 + lane / 4;
-        b_src[q] = (uint32_t)((row < b_last ? row : b_last) * steps * 64 + 16 * ((lane % 4) ^ mx_swizzle<64>(row)));
+        constexpr int lanes = P::BROW / 16;
+        const int row = (q * P::WAVES + wave) % P::B_PIECES * (64 / lanes) + lane / lanes;
+        const int at = 16 * ((lane % lanes) ^ mx_swizzle<P::BROW>(row));
+        b_src[q] = (uint32_t)((row < b_last ? row : b_last) * steps * 64 + at);
+        b_step[q] = at / 64 * 64;
     }
     const uint32_t *const as_tile = As + (int64_t)m0 * steps, *const bs_tile = Bs + (int64_t)n0 * steps;
 #pragma unroll
@@ -302,15 +315,19 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
             }
         }
     };
-    const auto load_stage = [&](int s) {
-        uint8_t *to = lds + (s % P::kBuffers) * P::kStage;
-        const int at = s < steps ? s : steps - 1;                        // past the end: the same number of loads
+    const int stages = (steps + S - 1) / S;
+    const auto load_stage = [&](int t) {
+        uint8_t *to = lds + (t % P::kBuffers) * P::kStage;
+        const int at = t < stages ? t : stages - 1;                      // past the end: the same number of loads
+        const bool half = S == 2 && S * at + 1 == steps;                 // a last step without a second: itself again
 #pragma unroll
         for (int q = 0; q < P::A_LOADS; q++)
-            mx_to_lds16(a_tile + at * P::ABYTES + a_src[q], to + (q * P::WAVES + wave) % P::A_PIECES * 1024);
+            mx_to_lds16(a_tile + at * P::AROW + (a_src[q] - (half ? a_step[q] : 0)),
+                        to + (q * P::WAVES + wave) % P::A_PIECES * 1024);
 #pragma unroll
         for (int q = 0; q < P::B_LOADS; q++)
-            mx_to_lds16(b_tile + at * 64 + b_src[q], to + P::TM * P::ABYTES + (q * P::WAVES + wave) % P::B_PIECES * 1024);
+            mx_to_lds16(b_tile + at * P::BROW + (b_src[q] - (half ? b_step[q] : 0)),
+                        to + P::TM * P::AROW + (q * P::WAVES + wave) % P::B_PIECES * 1024);
     };
     mx_v4f acc[MT][NT];
 #pragma unroll
@@ -318,24 +335,26 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = mx_v4f{0.f, 0.f, 0.f, 0.f};
     const int a_row = wm * MT * 16 + r16, b_row = wn * NT * 16 + r16;
-    const int a_off0 = a_row * P::ABYTES + 16 * (g ^ mx_swizzle<P::ABYTES>(r16));
-    const int a_off1 = a_row * P::ABYTES + 16 * ((g + 4) ^ mx_swizzle<P::ABYTES>(r16));
-    const int b_off = P::TM * P::ABYTES + b_row * 64 + 16 * (g ^ mx_swizzle<64>(r16));
+    // piece g of the first step; another piece's number is XORed onto it
+    const int a_off = a_row * P::AROW + 16 * (g ^ mx_swizzle<P::AROW>(r16));
+    const int b_off = P::TM * P::AROW + b_row * P::BROW + 16 * (g ^ mx_swizzle<P::BROW>(r16));
     mx_v4i fa[MT][FP8 ? 2 : 1], fb[NT];
     int sa[MT], sb[NT];
-    const auto fetch = [&](int s) {
-        const uint8_t *buf = lds + (s % P::kBuffers) * P::kStage;
+    const auto fetch = [&](int t, int h) {                               // step h of stage t
+        const uint8_t *buf = lds + (t % P::kBuffers) * P::kStage;
+        const int s = S * t + h;
         const uint8_t *sc = scales + ((s >> 2) & 1) * P::kScales + (s & 3) * s_step;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            fb[j] = *reinterpret_cast<const mx_v4i *>(buf + b_off + j * 16 * 64);
+            fb[j] = *reinterpret_cast<const mx_v4i *>(buf + (b_off ^ 64 * h) + j * 16 * P::BROW);
             sb[j] = (int)(*reinterpret_cast<const uint32_t *>(sc + (P::TM + b_row + 16 * j) * s_row) >> (8 * g));
         }
 #pragma unroll
         for (int i = 0; i < MT; i++) {
             sa[i] = (int)(*reinterpret_cast<const uint32_t *>(sc + (a_row + 16 * i) * s_row) >> (8 * g));
-            fa[i][0] = *reinterpret_cast<const mx_v4i *>(buf + a_off0 + i * 16 * P::ABYTES);
-            if constexpr (FP8) fa[i][1] = *reinterpret_cast<const mx_v4i *>(buf + a_off1 + i * 16 * P::ABYTES);
+            fa[i][0] = *reinterpret_cast<const mx_v4i *>(buf + (a_off ^ P::ABYTES * h) + i * 16 * P::AROW);
+            if constexpr (FP8)
+                fa[i][1] = *reinterpret_cast<const mx_v4i *>(buf + (a_off ^ P::ABYTES * h ^ 64) + i * 16 * P::AROW);
         }
     };
     const auto multiply = [&]() {
@@ -359,51 +378,58 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
     if constexpr (P::WAVES == 8) {
         // Two waves per SIMD, one of each half of the workgroup, half a step apart: while one half reads its fragments
         // the other multiplies.  A phase ends with a barrier; half 0 reads step s in phase 2 s and multiplies in phase
-        // 2 s + 1, half 1 a phase later.  The stage asked for in the phase that reads step s goes to the buffer that held
-        // stage s - 1, which both halves have read by the end of phase 2 s - 1.  Stage s + 1 has to be there at the
-        // end of phase 2 s + 1, where half 0 has multiplied step s and half 1 has read it.
+        // 2 s + 1, half 1 a phase later.  A stage asked for in the phase that reads the first step of stage t goes to the
+        // buffer that held stage t - 1, which both halves had read by the end of the phase before.  Stage t + 1 has to be
+        // there at the end of the phase in which half 0 has multiplied the last step of stage t and half 1 has read it.
         const bool half1 = wave >= 4;
         mx_wait_loads<P::wait(false)>();
         __builtin_amdgcn_s_barrier();
         if (half1) __builtin_amdgcn_s_barrier();
-        for (int s = 0; s < steps; s++) {
-            const bool group = (s & 3) == 0;
-            if (group) load_scales((s >> 2) + 1);
-            load_stage(s + P::kAhead);
-            fetch(s);
-            if (half1) {
-                if (group) mx_wait_loads<P::wait(true)>();
-                else mx_wait_loads<P::wait(false)>();
-            } else {
-                mx_wait_lds();
-            }
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_s_setprio(1);
-            multiply();
-            // the products belong to this phase (nothing else keeps them on this side of the barrier)
+        for (int t = 0; t < stages; t++) {
+            const bool group = (S * t & 3) == 0;
+            if (group) load_scales((S * t >> 2) + 1);
+            load_stage(t + P::kAhead);
 #pragma unroll
-            for (int i = 0; i < MT; i++)
+            for (int h = 0; h < S; h++) {
+                if (h && S * t + h == steps) break;
+                const bool last = h == S - 1 || S * t + h + 1 == steps;
+                const auto arrive = [&]() {
+                    if (last && group) mx_wait_loads<P::wait(true)>();
+                    else if (last) mx_wait_loads<P::wait(false)>();
+                    else mx_wait_lds();
+                };
+                fetch(t, h);
+                if (half1) arrive();
+                else mx_wait_lds();
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_s_setprio(1);
+                multiply();
+                // the products belong to this phase (nothing else keeps them on this side of the barrier)
 #pragma unroll
-                for (int j = 0; j < NT; j++) asm volatile("" : "+v"(acc[i][j]));
-            __builtin_amdgcn_s_setprio(0);
-            if (!half1) {
-                if (group) mx_wait_loads<P::wait(true)>();
-                else mx_wait_loads<P::wait(false)>();
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) asm volatile("" : "+v"(acc[i][j]));
+                __builtin_amdgcn_s_setprio(0);
+                if (!half1 && last) arrive();
+                __builtin_amdgcn_s_barrier();
             }
-            __builtin_amdgcn_s_barrier();
         }
         if (!half1) __builtin_amdgcn_s_barrier();
     } else {
-        // Step s: stage s has arrived, for this wave (the wait) and for all (the barrier), behind which all waves are also
-        // done with the buffer of stage s - 1, which takes the next one.  Other workgroups of the CU fill the waits.
+        // Stage t has arrived, for this wave (the wait) and for all (the barrier), behind which all waves are also done with
+        // the buffer of stage t - 1, which takes the next one.  Other workgroups of the CU fill the waits.
         mx_wait_loads<P::wait(false)>();
-        for (int s = 0; s < steps; s++) {
-            const bool group = (s & 3) == 0;
+        for (int t = 0; t < stages; t++) {
+            const bool group = (S * t & 3) == 0;
             __builtin_amdgcn_s_barrier();
-            if (group) load_scales((s >> 2) + 1);
-            load_stage(s + P::kAhead);
-            fetch(s);
-            multiply();
+            if (group) load_scales((S * t >> 2) + 1);
+            load_stage(t + P::kAhead);
+#pragma unroll
+            for (int h = 0; h < S; h++) {
+                if (h && S * t + h == steps) break;
+                fetch(t, h);
+                multiply();
+            }
             if (group) mx_wait_loads<P::wait(true)>();
             else mx_wait_loads<P::wait(false)>();
         }
@@ -431,13 +457,13 @@ struct MmArgs {
     hipStream_t st;
 };
 
-template <bool FP8, typename O, int WM, int WN, int MT, int NT, int BUFFERS>
+template <bool FP8, typename O, int WM, int WN, int MT, int NT, int S, int BUFFERS>
 static int mm_tile_launch(const MmArgs &a, const char *who)
 {
-    using P = MxTile<FP8, WM, WN, MT, NT, BUFFERS>;
+    using P = MxTile<FP8, WM, WN, MT, NT, S, BUFFERS>;
     const int64_t mt = ceil_div(a.M, P::TM), nt = ceil_div(a.N, P::TN);
     NB_REQUIRE(mt * nt < (1 << 21) && a.steps <= P::kMaxSteps, "%s: too many tiles", who);
-    auto *kernel = mx_mm_tile_kernel<FP8, O, WM, WN, MT, NT, BUFFERS>;
+    auto *kernel = mx_mm_tile_kernel<FP8, O, WM, WN, MT, NT, S, BUFFERS>;
     static std::atomic<uint64_t> ready{0};              // devices on which the kernel's LDS size has been set
     int device = 0;
     (void)hipGetDevice(&device);
@@ -465,9 +491,9 @@ static int mm_rows_launch(const MmArgs &a, const char *who, int rm = 16, int rn 
 // has at most one workgroup (a step's latency), `full` for 256 workgroups of a launch that fills the card many times over.
 // Measured at K = 8192, in microseconds, E4M3 / E2M1:
 //                        256x256      128x128     64x128      64x64       16x64       16x32       16x16
-//   4096 x 16384        702 / 275    902 / 373   961 / 517  1070 / 716
-//   4096 x 1024         165 /  64     77 /  34    63 /  37    72 /  48
-//   1024 x 1024         163 /  63     75 /  32    42 /  23    29 /  18
+//   4096 x 16384        702 / 272    902 / 373   961 / 517  1070 / 716
+//   4096 x 1024         165 /  61     77 /  34    63 /  37    72 /  48
+//   1024 x 1024         163 /  59     75 /  32    42 /  23    29 /  18
 //    256 x 1024                                   42 /  22    29 /  18    18 /  14    21 /  16    27 /  19
 //     64 x 1024                                   42 /  22    29 /  18    18 /  14    12 /   9     9 /   7
 //     16 x 32768                                  45 /  24    43 /  24    31 /  26    38 /  31    52 / -
@@ -523,10 +549,10 @@ static int mm_launch(const MmArgs &a, const char *who)
 {
     const MmPlan plan = mm_plan(a, FP8);
     switch (plan.kind) {
-        case 0: return mm_tile_launch<FP8, O, 4, 2, 4, 8, FP8 ? 3 : 4>(a, who);
-        case 1: return mm_tile_launch<FP8, O, 2, 2, 4, 4, 3>(a, who);
-        case 2: return mm_tile_launch<FP8, O, 2, 2, 2, 4, 4>(a, who);
-        case 3: return mm_tile_launch<FP8, O, 4, 1, 1, 4, 4>(a, who);
+        case 0: return mm_tile_launch<FP8, O, 4, 2, 4, 8, FP8 ? 1 : 2, FP8 ? 3 : 2>(a, who);
+        case 1: return mm_tile_launch<FP8, O, 2, 2, 4, 4, 1, 3>(a, who);
+        case 2: return mm_tile_launch<FP8, O, 2, 2, 2, 4, 1, 4>(a, who);
+        case 3: return mm_tile_launch<FP8, O, 4, 1, 1, 4, 1, 4>(a, who);
         case 4: return mm_rows_launch<FP8, O, 1, 4, 4>(a, who);
         case 5: return mm_rows_launch<FP8, O, 1, 2, 4>(a, who);
         default: return mm_rows_launch<FP8, O, 1, 1, 8>(a, who, plan.rm, plan.rn);
