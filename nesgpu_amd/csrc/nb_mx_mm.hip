@@ -462,7 +462,7 @@ static int mm_tile_launch(const MmArgs &a, const char *who)
 {
     using P = MxTile<FP8, WM, WN, MT, NT, S, BUFFERS>;
     const int64_t mt = ceil_div(a.M, P::TM), nt = ceil_div(a.N, P::TN);
-    NB_REQUIRE(mt * nt < (1 << 21) && a.steps <= P::kMaxSteps, "%s: too many tiles", who);
+    NB_REQUIRE(mt * nt <= (1LL << 31) / (64 * P::WAVES) && a.steps <= P::kMaxSteps, "%s: too many tiles", who);
     auto *kernel = mx_mm_tile_kernel<FP8, O, WM, WN, MT, NT, S, BUFFERS>;
     static std::atomic<uint64_t> ready{0};              // devices on which the kernel's LDS size has been set
     int device = 0;
@@ -534,7 +534,7 @@ static MmPlan mm_plan(const MmArgs &a, bool fp8)
     const double touched = 0.00032 * pieces(plan.rm, plan.rn);
     double least = std::max(0.02 + touched, (0.04 + touched) * (tiles(plan.rm, plan.rn) / 256.0));
     for (int v = 0; v < 6; v++) {
-        if (v < 4 && a.steps > 65536) continue;                  // longer rows than the tiles' offsets reach
+        if (v < 4 && a.steps >= 65536) continue;                 // longer rows than the tiles' offsets reach
         const MmCost &c = kMmCosts[fp8][v];
         double rounds = (double)ceil_div(a.M, c.rows) * (double)ceil_div(a.N, c.columns) / 256.0;
         if (c.one_per_cu) rounds = ceil(rounds);

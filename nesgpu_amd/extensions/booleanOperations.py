@@ -1327,7 +1327,7 @@ class MXRows:
         self = cls.__new__(cls)
         self._code_bytes = padded // _MX_FORMATS[format][1]
         self._codes = None
-        self._scales = torch.empty((rows * (self._code_bytes + padded // 32),), dtype=torch.uint8, device=device)
+        self._scales = torch.empty(rows * (self._code_bytes + padded // 32), dtype=torch.uint8, device=device)
         self._device = device
         self.rows, self.K, self.format = rows, K, format
         return self
@@ -1340,9 +1340,10 @@ class MXRows:
 
     def _parts(self):
         if self._codes is None:
-            both, n = self._scales, self.rows * self._code_bytes
-            self._codes = both[:n].view(self.rows, self._code_bytes)
-            self._scales = both[n:].view(self.rows, -1) if self.rows else both.view(0, ceil_div(self.K, _MX_STEP) * 4)
+            both, rows, n = self._scales, self.rows, self._code_bytes
+            per_row = ceil_div(self.K, _MX_STEP) * (_MX_STEP // 32)
+            self._codes = both.as_strided((rows, n), (n, 1))
+            self._scales = both.as_strided((rows, per_row), (per_row, 1), rows * n)
         return self._codes, self._scales
 
     @property
@@ -1388,7 +1389,7 @@ def mx_dequantize(rows, dtype=torch.bfloat16):
     """The values that :class:`MXRows` stand for, [rows, K] in ``dtype`` (float32, float16 or bfloat16; one rounding, and
     none for float32, or for bfloat16 above its subnormals)."""
     assert isinstance(rows, MXRows)
-    out = torch.empty((rows.rows, rows.K), dtype=dtype, device=rows.device)
+    out = torch.empty_strided((rows.rows, rows.K), (rows.K, 1), dtype=dtype, device=rows._device)
     kind = _mx_type(out, "dtype")
     with _on(out):
         _lib.call("nb_mx_dequantize", out.data_ptr(), kind, *rows._pointers(),
@@ -1441,7 +1442,7 @@ def mx_mm_nt(A, B, dtype=torch.float32):
     if B.format != "fp4":
         raise NotImplementedError("the second operand must be in format 'fp4'")
     _same_device(A, B)
-    C = torch.empty((A.rows, B.rows), dtype=dtype, device=A.device)
+    C = torch.empty_strided((A.rows, B.rows), (B.rows, 1), dtype=dtype, device=A._device)
     kind = _mx_type(C, "dtype")
     if A.K == 0:
         return C.zero_()
@@ -1498,8 +1499,8 @@ def sample_tokens_from_words(logits, words, temperature=1.0, top_k=0, top_p=1.0,
     m_ptr, m = _row_setting(min_p, "min_p", torch.float32, R, dev)
     k = max(min(k, 2 ** 31 - 1), 0)
     need = _lib.load().nb_sample_tokens_workspace_bytes(R, V)
-    work = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    out = torch.empty((R,), dtype=torch.int32, device=dev)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    out = torch.empty(R, dtype=torch.int32, device=dev)
     with _on(logits):
         _lib.call("nb_sample_tokens", out.data_ptr(), logits.data_ptr(), kind, words.data_ptr(), t_ptr, t, k_ptr, k, p_ptr,
                   p, m_ptr, m, R, V, None if work is None else work.data_ptr(), need, _stream(logits))

@@ -704,3 +704,31 @@ def test_offsets_past_32_bits(ops):
     for kw in (dict(top_p=0.9), dict(temperature=0.0)):
         assert torch.equal(ops.sample_tokens_from_words(x, words, **kw)[-3:],
                            ops.sample_tokens_from_words(tail, words[-3:].contiguous(), **kw))
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+@pytest.mark.parametrize("K", [65535 * 128, 65536 * 128, 65537 * 128])
+def test_product_of_the_longest_rows(ops, K, a_format):
+    """Ones: every sum is K, a whole number below 2^24 that fp32 holds at each step."""
+    one = {"fp4": 0x22, "fp8": 0x38}
+
+    def rows(n, format):
+        return ops.MXRows(torch.full((n, K // (2 if format == "fp4" else 1)), one[format], dtype=torch.uint8, device="cuda"),
+                          torch.full((n, K // 32), 127, dtype=torch.uint8, device="cuda"), K, format)
+
+    for M, N in ((300, 70), (2, 5)):
+        got = ops.mx_mm_nt(rows(M, a_format), rows(N, "fp4"))
+        assert bool((got == K).all())
+
+
+@pytest.mark.parametrize("a_format", O.FORMATS)
+def test_product_of_very_many_rows(ops, a_format):
+    """More tiles of one operand than fit 16 + 5 bits."""
+    M, N, K = 200_000_003, 3, 1
+    A = ops.MXRows(torch.zeros(M, 64 if a_format == "fp4" else 128, dtype=torch.uint8, device="cuda"),
+                   torch.full((M, 4), 127, dtype=torch.uint8, device="cuda"), K, a_format)
+    A.codes[-2:, 0] = 0x02 if a_format == "fp4" else 0x38
+    B = ops.mx_quantize(torch.tensor([[1.0], [-2.0], [3.0]], device="cuda"), "fp4")
+    got = ops.mx_mm_nt(A, B, torch.bfloat16)
+    assert not bool(got[:-2].any())
+    assert got[-2:].tolist() == [[1.0, -2.0, 3.0]] * 2
