@@ -5,14 +5,15 @@
 // row's maximum names the bin the border lies in, and only that bin's entries are looked at digit by digit.  Weights are
 // integers (a weight of 1 is 2^f): sums over a row are the same in any order, and are accumulated with atomics.
 //
-// Rows of at most 64 entries: a wave per row, ranks by comparing all pairs.  Up to 16384: a workgroup per row.  Longer
+// Rows of at most 64 entries: a wave per row, ranks by comparing all pairs.  Up to 16376: a workgroup per row.  Longer
 // ones: one kernel over chunks of 8192 entries (the exponentials, which bound the whole, are then spread over the card
 // however few the rows), one workgroup per row to finish from the chunks' histograms.
 //
 // What bounds it: rows of up to 16376 entries and few rows of any length, the latency of about ten phases that follow each
 // other (a phase 1 to 4 us, most of it waiting for one workgroup's instructions and for memory); 256 x 131072 bf16 with a
-// cut, 90 us: 48 us the exponentials' kernel (37 instructions an entry, two thirds of the cycles), 42 us the rows' kernel, 10
-// of them the second look at every logit at what the last cache gives to all CUs (7 TB/s).
+// cut, 93 us: 48 us the exponentials' kernel (37 instructions an entry, two thirds of the cycles), 45 us the rows' kernel, 10
+// of them the second look at every logit at what the last cache gives to all CUs (7 TB/s).  A border's bin of more entries
+// than the list holds costs a pass over the row per digit: 4 x 131072 equal logits 518 us, of N(0, 0.001^2) 298 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,7 +31,6 @@ constexpr int kTokenMaxChunks = kTokenMaxV / (kGroup * kChunkGroups) + 1;
 constexpr int kSlots = 256;                          // bins of 1/8 of an octave of the weights below the maximum; the last
                                                      // one holds all that is further below
 constexpr int kSlotsPerOctave = 8;
-constexpr uint32_t kTokenList = 4096;                     // entries of a border bin that fit LDS
 
 // Order-preserving keys; 0: an entry that is never drawn (NaN, -inf; no int32 entry is).  -0 and +0 are one key.
 __device__ __forceinline__ uint32_t token_key(float v)
@@ -41,6 +41,8 @@ __device__ __forceinline__ uint32_t token_key(float v)
 }
 template <typename T>
 struct TokenKey {
+    // bits at a key's end that are clear in positive logits' keys and set in negative ones'
+    static constexpr int kFree = __is_same(T, Bf16) ? 16 : __is_same(T, _Float16) ? 13 : 0;
     static __device__ __forceinline__ bool drawable(uint32_t k) { return k != 0; }
     static __device__ __forceinline__ double value(uint32_t k)
     {
@@ -93,6 +95,7 @@ struct TokenKey {
 };
 template <>
 struct TokenKey<int32_t> {
+    static constexpr int kFree = 0;
     static __device__ __forceinline__ bool drawable(uint32_t) { return true; }
     static __device__ __forceinline__ double value(uint32_t k) { return (double)(int32_t)(k ^ 0x80000000u); }
     static __device__ __forceinline__ uint32_t key1(const int32_t *p) { return (uint32_t)*p ^ 0x80000000u; }
@@ -295,14 +298,14 @@ struct TokenScale {
         const uint32_t d = ((uint32_t)last - step) / kStepsPerBin;
         return alone || d >= kSlots ? kSlots - 1 : (int)d;
     }
-    // keys that can lie in a slot, a little more than those that do: from ... to
+    // keys that can lie in a slot, a little more than those that do: from ... to; of the last one those that have a weight
     __device__ __forceinline__ void window(int s, uint32_t &from, uint32_t &to) const
     {
-        from = 0, to = kmax;
+        from = kmax, to = kmax;                          // alone: no other has a weight
         if (alone) return;
         const double end = (fma(vmax, rate256, kExpHalf) - kExpHalf) + (double)(last & (kStepsPerBin - 1)) -
                            (double)(token_low(fma(vmax, rate256, kExpHalf)) & (kStepsPerBin - 1)) - (double)(s * kStepsPerBin);
-        if (s < kSlots - 1) from = TokenKey<T>::below((end - kStepsPerBin + 0.5) / rate256);
+        from = TokenKey<T>::below(s < kSlots - 1 ? (end - kStepsPerBin + 0.5) / rate256 : vmax - (frac + 1) * (double)kExpTable / rate256);
         const uint32_t above = s ? TokenKey<T>::above((end + 0.5) / rate256) : kmax;
         to = above < kmax ? above : kmax;
     }
@@ -566,17 +569,19 @@ struct TokenEntry {
 };
 
 template <typename T, int THREADS, int HELD>
-__global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
+__global__ __launch_bounds__(THREADS, 4) void sample_row_kernel(TokenArgs a)
 {
     constexpr bool LOCAL = HELD > 0;
     constexpr int WAVES = THREADS / 64;
     constexpr int SEGS = LOCAL ? kTokenLocalV / (kGroup * kSegGroups) + 1 : kTokenMaxSegs;
     constexpr int CHUNKS = LOCAL ? 1 : kTokenMaxChunks;
-    constexpr uint32_t kList = LOCAL ? 1024 : kTokenList;
+    constexpr uint32_t kList = LOCAL ? 1024 : 8 * THREADS;   // entries of a border's bin that fit LDS
     __shared__ TokenExp table;
     __shared__ TokenEdges edges;
-    __shared__ uint64_t seg_w[SEGS];                     // what is kept of a segment; tie counts and indexes before
-    static_assert(LOCAL || sizeof(seg_w) >= kList * sizeof(uint32_t), "room for a list's indexes");
+    // what is kept of a segment, tie counts before; of long rows the groups that have an entry in the border's bin, and the
+    // indexes of those that tie, before either
+    __shared__ uint64_t seg_w[LOCAL || SEGS > (int)kList / 2 ? SEGS : kList / 2];
+    uint32_t *const found = reinterpret_cast<uint32_t *>(seg_w);
     __shared__ double slot_w[kSlots];
     __shared__ uint64_t hist_w[kSlots];                  // LOCAL: by slot; later by digit
     __shared__ uint32_t hist_c[kSlots], slot_c[kSlots];
@@ -765,6 +770,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
         }
         __syncthreads();
         // ---- the borders, one after the other: top_k, top_p, min_p -----------------------------------------------------
+        uint32_t from = 0, to = 0;                       // the window of keys around the last border's slot
         double total = 0.0;                              // what top_p is a part of
         bool have_total = false;
 #pragma unroll 1
@@ -813,7 +819,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
             if (slot < 0 || slot > border) continue;     // the row has no more than that: nothing is cut
             if (slot != border || !listed) {             // else the list of the border before is the one
                 // keys that can lie there, a little more than those that do
-                uint32_t from, to;
                 scale.window(slot, from, to);
                 // the entries of a group that lie in the slot, into the list
                 const auto put = [&](const uint32_t (&keys)[8], uint32_t have, int i0) {
@@ -839,7 +844,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                     // entry, then, a thread each, for the entries.  (Entry by entry at once, a wave goes through all of that
                     // for the few of its lanes that have one: 17 us more for 131072 entries.)
                     constexpr int WORDS = sizeof(T) / 2, AHEAD = 8 / WORDS;      // 16-byte words of a group
-                    uint32_t *const found = reinterpret_cast<uint32_t *>(seg_w);
                     const typename TokenKey<T>::Near near(from, to);
 #pragma unroll 1
                     for (int s = wave; s < segs; s += AHEAD * WAVES) {
@@ -883,6 +887,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                 border = slot;
             }
             if (which == 2) continue;                    // the entries below min_key stay out by their keys
+            if (list_n == 0) continue;                   // nothing with a weight below the slots before: nothing is cut
             if (list_n <= 64) {
                 // few enough for a lane each: what lies above an entry, by comparing all pairs (every wave does the same)
                 const uint32_t q = (uint32_t)lane < list_n ? list[lane].key : 0u;
@@ -908,10 +913,11 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                 before_c += __shfl(above_c, l);
                 before_w += (double)__shfl(above_w, l);
             } else {
-                // Digit by digit among the slot's keys, from the list or, where it has too many, from memory every time; only
-                // the bits in which the list's keys differ (logits of 16 bits have few).
-                int top_bit = 32, low_bit = 0;
-                uint32_t prefix = 0;
+                // Digit by digit among the slot's keys, from the list or, where it has too many, from the row every time; only
+                // the bits in which the list's keys differ (logits of 16 bits have few) or the window's.
+                int top_bit = from ^ to ? 32 - __builtin_clz(from ^ to) : 1, low_bit = TokenKey<T>::kFree;
+                if (top_bit <= low_bit) top_bit = low_bit + 1;
+                uint32_t prefix = top_bit < 32 ? from >> top_bit : 0;
                 if (listed) {
                     uint32_t both = 0xFFFFFFFFu, one = 0;
                     for (uint32_t i = tid; i < list_n; i += THREADS) both &= list[i].key, one |= list[i].key;
@@ -926,8 +932,6 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                     low_bit = differ ? __builtin_ctz(differ) : 0;
                     prefix = top_bit < 32 ? both >> top_bit : 0;
                 }
-                // bits below low_bit are the same in all keys
-                const uint32_t rest = listed ? list[0].key & ((1u << low_bit) - 1u) : 0u;
 #pragma unroll 1
                 for (int shift = top_bit; shift > low_bit;) {
                     const int width = shift - low_bit < 8 ? shift - low_bit : 8;
@@ -935,7 +939,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                     __syncthreads();
                     for (int t = tid; t < kSlots; t += THREADS) hist_w[t] = 0, hist_c[t] = 0;
                     __syncthreads();
-                    const auto put = [&](uint32_t q) {
+                    const auto add = [&](uint32_t q) {
                         if (shift + width == 32 || q >> (shift + width) == prefix) {
                             const uint32_t d = (q >> shift) & ((1u << width) - 1u);
                             atomicAdd(&hist_c[d], 1u);
@@ -943,23 +947,21 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                         }
                     };
                     if (listed) {
-                        for (uint32_t i = tid; i < list_n; i += THREADS) put(list[i].key);
-                    } else if constexpr (LOCAL) {
-#pragma unroll
-                        for (int q = 0; q < HELD; q++)
-#pragma unroll 1
-                            for (uint32_t left = held_have[q]; left; left &= left - 1) {
-                                uint32_t k = held[q][0];
-#pragma unroll
-                                for (int d = 1; d < 8; d++) k = d == __builtin_ctz(left) ? held[q][d] : k;
-                                if (scale.slot(k) == slot) put(k);
-                            }
+                        for (uint32_t i = tid; i < list_n; i += THREADS) add(list[i].key);
                     } else {
+                        for_groups(one_ahead, 0, segs, [&](const uint32_t (&keys)[8], uint32_t have, int, int) {
+                            uint32_t near = 0;
+#pragma unroll
+                            for (int e = 0; e < 8; e++) near |= (uint32_t)(keys[e] >= from && keys[e] <= to) << e;
 #pragma unroll 1
-                        for (int i = tid; i < a.V; i += THREADS) {
-                            const uint32_t q = TokenKey<T>::key1(x.row + i);
-                            if (TokenKey<T>::drawable(q) && scale.slot(q) == slot) put(q);
-                        }
+                            for (near &= have; near; near &= near - 1) {
+                                const int e = __builtin_ctz(near);
+                                uint32_t k = keys[0];
+#pragma unroll
+                                for (int d = 1; d < 8; d++) k = d == e ? keys[d] : k;
+                                if (scale.slot(k) == slot) add(k);
+                            }
+                        });
                     }
                     __syncthreads();
                     if (wave == 0) {                     // lane l: the digits 255 - 4 l down to 252 - 4 l
@@ -997,7 +999,9 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
                     equal = sh_ties;
                     prefix = (prefix << width) | (uint32_t)sh_at;
                 }
-                key = (prefix << low_bit) | rest;
+                // bits below low_bit are the same in all keys, or, of 16-bit types, go with the sign
+                const uint32_t rest = (1u << low_bit) - 1u;
+                key = (prefix << low_bit) | (rest & (listed ? list[0].key : prefix >> (31 - low_bit) & 1 ? 0u : ~0u));
             }
             // the ties of `key` that are kept, before_c entries or before_w of weight lying above them
             const uint64_t w = scale.weight(key);
@@ -1022,19 +1026,18 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(TokenArgs a)
     int last = a.V;
     if (!LOCAL && listed && ties < equal && key >= lowest) {
         // all entries equal to `key` are in the list: the one with ties - 1 of them before it
-        uint32_t *const same = reinterpret_cast<uint32_t *>(seg_w);
         __syncthreads();
         if (tid == 0) sh_n = 0;
         __syncthreads();
         for (uint32_t i = tid; i < list_n; i += THREADS)
-            if (list[i].key == key) same[atomicAdd(&sh_n, 1u)] = (uint32_t)list[i].index;
+            if (list[i].key == key) found[atomicAdd(&sh_n, 1u)] = (uint32_t)list[i].index;
         __syncthreads();
         const uint32_t n = sh_n;
         for (uint32_t i = tid; i < n; i += THREADS) {
-            const uint32_t mine = same[i];
+            const uint32_t mine = found[i];
             uint32_t before = 0;
 #pragma unroll 8
-            for (uint32_t j = 0; j < n; j++) before += same[j] < mine;
+            for (uint32_t j = 0; j < n; j++) before += found[j] < mine;
             if (before == ties - 1) sh_at = (int)mine;
         }
         __syncthreads();
@@ -1208,25 +1211,38 @@ static int token_chunks(int64_t V) { return (int)ceil_div(V + kGroup - 1, kChunk
 template <typename T>
 static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
 {
-    // Borders, in microseconds without a cut / with top_p = 0.9, logits N(0, 2.5^2), this kernel and the one for longer rows:
-    //   4096 x 64 fp32        9 /  15      23 /  46
-    //   1024 x 2000 bf16     10 /  21      26 /  65
-    //    256 x 8000 bf16      9 /  26      16 /  35 (by chunks)
+    // Borders, in microseconds without a cut / with top_p = 0.9, logits N(0, 2.5^2), this kernel / the one on the other side:
+    //   4096 x 64 fp32        9 /  15      23 /  46 (a workgroup per row)
+    //   1024 x 2000 bf16     10 /  21      26 /  65 (1024 threads)
+    //    100 x 4000 bf16      9 /  18       9 /  21 (1024 threads)
+    //    200 x 8000 bf16     10 /  25       9 /  27 (1024 threads of one group)
+    //    600 x 8000 bf16      - /  49       - /  71
     //    256 x 16000 bf16    13 /  28      18 /  37 (by chunks)
-    //   1024 x 16000 fp32    52 / 111      69 / 134 (by chunks)
-    // By chunks: 64 x 32768 bf16 17 / 32, 1 x 131072 bf16 16 / 38, 256 x 131072 bf16 51 / 90, the largest entry alone 20.
-    if (a.V <= 64)
+    //     10 x 16000 fp32    12 /  29      14 /  31 (512 threads of four groups: two workgroups a CU, so for more rows than CUs)
+    //   1024 x 16000 fp32    39 /  83      50 / 115 (1024 threads of two)
+    //   1024 x 32768 bf16    82 / 113      82 / 160 (1024 threads, one workgroup a CU)
+    //    400 x 131072 bf16    - / 155       - / 161 (512 threads), 1 x 131072 fp32 16 / 37, 16 / 43
+    // By chunks also: 64 x 32768 bf16 17 / 31, 5 x 50001 fp16 17 / 32, 256 x 131072 bf16 51 / 93, the largest entry alone 20.
+    const dim3 rows((unsigned)a.R);
+    if (a.V <= 64) {
         sample_short_kernel<T><<<dim3((unsigned)ceil_div(a.R, 4)), dim3(256), 0, st>>>(a);
-    else if (a.V <= 256 * kGroup - 8)                    // a row that starts inside a group reaches into one more
-        sample_row_kernel<T, 256, 1><<<dim3((unsigned)a.R), dim3(256), 0, st>>>(a);
-    else if (a.V <= 1024 * kGroup - 8)
-        sample_row_kernel<T, 1024, 1><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
-    else if (a.V <= kTokenLocalV)
-        sample_row_kernel<T, 1024, 2><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
-    else {
+    } else if (a.V <= 256 * kGroup - 8) {                // a row that starts inside a group reaches into one more
+        sample_row_kernel<T, 256, 1><<<rows, dim3(256), 0, st>>>(a);
+    } else if (a.V <= 512 * kGroup - 8) {
+        sample_row_kernel<T, 512, 1><<<rows, dim3(512), 0, st>>>(a);
+    } else if (a.V <= 1024 * kGroup - 8) {
+        sample_row_kernel<T, 512, 2><<<rows, dim3(512), 0, st>>>(a);
+    } else if (a.V <= kTokenLocalV && a.R > 256) {
+        sample_row_kernel<T, 512, 4><<<rows, dim3(512), 0, st>>>(a);
+    } else if (a.V <= kTokenLocalV) {
+        sample_row_kernel<T, 1024, 2><<<rows, dim3(1024), 0, st>>>(a);
+    } else {
         token_chunk_kernel<T><<<dim3((unsigned)std::min<int64_t>(a.R * a.chunks, kChunkGrid)), dim3(512), 0, st>>>(a);
         if (const int rc = check_launch(who)) return rc;
-        sample_row_kernel<T, 1024, 0><<<dim3((unsigned)a.R), dim3(1024), 0, st>>>(a);
+        if (a.V <= 65536)
+            sample_row_kernel<T, 512, 0><<<rows, dim3(512), 0, st>>>(a);
+        else
+            sample_row_kernel<T, 1024, 0><<<rows, dim3(1024), 0, st>>>(a);
     }
     return check_launch(who);
 }
