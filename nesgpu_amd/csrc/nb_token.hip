@@ -575,7 +575,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_row_kernel(TokenArgs a)
     constexpr int WAVES = THREADS / 64;
     constexpr int SEGS = LOCAL ? kTokenLocalV / (kGroup * kSegGroups) + 1 : kTokenMaxSegs;
     constexpr int CHUNKS = LOCAL ? 1 : kTokenMaxChunks;
-    constexpr uint32_t kList = LOCAL ? 1024 : 8 * THREADS;   // entries of a border's bin that fit LDS
+    constexpr uint32_t kList = LOCAL && THREADS > 128 ? 1024 : 8 * THREADS;   // entries of a border's bin that fit LDS
     __shared__ TokenExp table;
     __shared__ TokenEdges edges;
     // what is kept of a segment, tie counts before; of long rows the groups that have an entry in the border's bin, and the
@@ -1212,7 +1212,9 @@ template <typename T>
 static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
 {
     // Borders, in microseconds without a cut / with top_p = 0.9, logits N(0, 2.5^2), this kernel / the one on the other side:
-    //   4096 x 64 fp32        9 /  15      23 /  46 (a workgroup per row)
+    //   4096 x 64 fp32        9 /  15      15 /  25 (64 threads)
+    //   5818 x 500 fp32       - /  29       - /  66 (256 threads), 10 x 500 12, 12
+    //   5338 x 741 bf16       - /  43       - /  68 (256 threads), 10 x 1000 14, 14
     //   1024 x 2000 bf16     10 /  21      26 /  65 (1024 threads)
     //    100 x 4000 bf16      9 /  18       9 /  21 (1024 threads)
     //    200 x 8000 bf16     10 /  25       9 /  27 (1024 threads of one group)
@@ -1226,7 +1228,11 @@ static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
     const dim3 rows((unsigned)a.R);
     if (a.V <= 64) {
         sample_short_kernel<T><<<dim3((unsigned)ceil_div(a.R, 4)), dim3(256), 0, st>>>(a);
-    } else if (a.V <= 256 * kGroup - 8) {                // a row that starts inside a group reaches into one more
+    } else if (a.V <= 64 * kGroup - 8) {                 // a row that starts inside a group reaches into one more
+        sample_row_kernel<T, 64, 1><<<rows, dim3(64), 0, st>>>(a);
+    } else if (a.V <= 128 * kGroup - 8) {
+        sample_row_kernel<T, 128, 1><<<rows, dim3(128), 0, st>>>(a);
+    } else if (a.V <= 256 * kGroup - 8) {
         sample_row_kernel<T, 256, 1><<<rows, dim3(256), 0, st>>>(a);
     } else if (a.V <= 512 * kGroup - 8) {
         sample_row_kernel<T, 512, 1><<<rows, dim3(512), 0, st>>>(a);
