@@ -192,9 +192,11 @@ __device__ __forceinline__ double row_sum(double s, double *part)
 // elements) stays in registers between the sum and the products; N = 0: rows of any length, read again for the products,
 // out of the caches for the most part.
 //
-// Bound by memory: with a residual in bf16 7 + 1/32 bytes an element, 8192 x 8192 in 92 to 102 us (4.6 to 5.1 TB/s; a large copy
-// 5.1).  The weights are loaded after the sum: taken before it they cost 16 registers per piece over the barrier and a
+// Bound by memory: with a residual in bf16 7 + 1/32 bytes an element, 8192 x 8192 in 92 to 102 us (4.6 to 5.1 TB/s; a large
+// copy 5.1).  The weights are loaded after the sum: taken before it they cost 16 registers per piece over the barrier and a
 // third of the waves (151 us).  Without a residual the 64-bit products show: 58 us for 3.0 bytes an element, 3.5 TB/s.
+// A wave per row, without barriers, up to 1024 elements: 32768 x 1024 bf16 41 us, 15530 x 547 23 us; a workgroup of 256
+// threads 52 and 34, of 128 43 and 24; four pieces a lane, up to 2048: 20000 x 1500 fp32 95 us, 79 with 256 threads.
 // One piece per thread: 8 waves a SIMD (64 registers) 16384 x 4096 90 us, 95 with 68 registers; two pieces need their 92.
 // Rows above 8192 are read twice: 4096 x 16384 bf16 105 us (held by 1024 threads of two pieces 107), 2000 x 32000 fp16
 // 107 us (of four pieces 131), 3355 x 20001 fp32 215 us (219).
@@ -326,6 +328,8 @@ static void norm_launch_vec(const NormArgs &a)
     const int64_t Kp = mx_padded(a.K);
     if (Kp <= 64 * 8)
         norm_launch_n<X, R, FP8, VEC, 64, 1>(a);
+    else if (Kp <= 64 * 16)
+        norm_launch_n<X, R, FP8, VEC, 64, 2>(a);
     else if (Kp <= 256 * 8)
         norm_launch_n<X, R, FP8, VEC, 256, 1>(a);
     else if (Kp <= 512 * 8)
