@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
 // What bounds it.  E2M1: the way from the second cache into LDS.  A tile of 256 x 256 takes 32 KB a step, of 128 x 128 16 KB,
 // and either arrives at 15 to 16 bytes a cycle and CU, however many stages are ahead (2, 3, 4 of 16 KB and 32 KB alike) and
 // however many CUs are at work (64, 256): 1.0 and 0.5 us a step, where the matrix instructions alone would take 0.45 and
-// 0.11.  8192 x 8192 x 8192 4.0 PFLOP/s.  E4M3: the matrix instructions, of which the split makes two, at 65 % of their rate.
+// 0.11.  8192 x 8192 x 8192 4.0 PFLOP/s.  E4M3: the matrix instructions, of which the split makes two, at 70 to 80 % of their rate.
 // Two steps a stage (128 bytes of every row, one stage ahead) are 2 to 5 % faster for 256 x 256 of E2M1: on random rows
 // 4096 x 16384 x 8192 306 us, 316 with one, 4096 x 8192 x 2048 52, 54.6; for the smaller tiles, whose waves have nobody to
 // take turns with, 10 to 20 % slower.
@@ -357,19 +357,40 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
                 fa[i][1] = *reinterpret_cast<const mx_v4i *>(buf + (a_off ^ P::ABYTES * h ^ 64) + i * 16 * P::AROW);
         }
     };
+    // E4M3: the smaller values of row set 0 before the products, those of the next set during this one's.  Left to itself the
+    // compiler puts a set's 48 mask operations before its 16 products, and the matrix unit waits; five of them after
+    // each product (three would do on average) are 633 us for 4096 x 16384 x 8192, four 647, six 643, as the compiler has it 707.
+    mx_v8i lo[2];
+    const auto prepare = [&]() {
+        mx_v8i hi;
+        if constexpr (FP8) mx_split<FP8>(lo[0], hi, fa[0][0], fa[0][FP8 ? 1 : 0]);
+    };
     const auto multiply = [&]() {
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            mx_v8i lo, hi;
-            mx_split<FP8>(lo, hi, fa[i][0], fa[i][FP8 ? 1 : 0]);
+            mx_v8i hi;
             if constexpr (FP8) {
 #pragma unroll
                 for (int j = 0; j < NT; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(lo, mx_wide(fb[j]), acc[i][j], 0, 4, 0, sa[i], 0, sb[j]);
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(lo[i & 1], mx_wide(fb[j]), acc[i][j], 0, 4, 0, sa[i], 0, sb[j]);
+                hi = __builtin_shufflevector(fa[i][0], fa[i][1], 0, 1, 2, 3, 4, 5, 6, 7) ^ lo[i & 1];
+                if (i + 1 < MT) {
+                    mx_v8i later;
+                    mx_split<FP8>(lo[(i + 1) & 1], later, fa[i + 1][0], fa[i + 1][1]);
+                }
+            } else {
+                hi = mx_wide(fa[i][0]);
             }
 #pragma unroll
             for (int j = 0; j < NT; j++)
                 acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(hi, mx_wide(fb[j]), acc[i][j], FP8 ? 0 : 4, 4, 0, sa[i], 0, sb[j]);
+        }
+        if constexpr (FP8 && P::WAVES == 8) {
+#pragma unroll
+            for (int i = 0; i < 2 * MT * NT; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                 // a matrix instruction,
+                __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);                 // five vector ones
+            }
         }
     };
     load_scales(0);
@@ -401,6 +422,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
                 fetch(t, h);
                 if (half1) arrive();
                 else mx_wait_lds();
+                prepare();
+                if constexpr (FP8) asm volatile("" : "+v"(lo[0]));               // on this side of the barrier
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_s_setprio(1);
                 multiply();
@@ -428,6 +451,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_mm_tile_kernel(O *__restrict_
             for (int h = 0; h < S; h++) {
                 if (h && S * t + h == steps) break;
                 fetch(t, h);
+                prepare();
                 multiply();
             }
             if (group) mx_wait_loads<P::wait(true)>();
@@ -488,12 +512,14 @@ static int mm_rows_launch(const MmArgs &a, const char *who, int rm = 16, int rn 
 }
 
 // Which kernel: the one whose time is least by two measured costs, in microseconds per step of K: `alone` where every CU
-// has at most one workgroup (a step's latency), `full` for 256 workgroups of a launch that fills the card many times over.
+// has at most one workgroup (a step's latency), `full` for 256 workgroups of a launch that fills the card many times over;
+// tiles are alike, so they come in whole rounds of 256 (2738 x 1951 x 9540 E4M3, 352 tiles of 128 x 128 147 us, 688 of 64 x 128
+// 123).
 // Measured at K = 8192, in microseconds, E4M3 / E2M1:
 //                        256x256      128x128     64x128      64x64       16x64       16x32       16x16
-//   4096 x 16384        702 / 272    902 / 373   961 / 517  1070 / 716
-//   4096 x 1024         165 /  61     77 /  34    63 /  37    72 /  48
-//   1024 x 1024         163 /  59     75 /  32    42 /  23    29 /  18
+//   4096 x 16384        631 / 272    860 / 373   947 / 517  1032 / 716
+//   4096 x 1024         135 /  61     74 /  34    63 /  37    73 /  48
+//   1024 x 1024         133 /  59     72 /  32    43 /  23    30 /  18
 //    256 x 1024                                   42 /  22    29 /  18    18 /  14    21 /  16    27 /  19
 //     64 x 1024                                   42 /  22    29 /  18    18 /  14    12 /   9     9 /   7
 //     16 x 32768                                  45 /  24    43 /  24    31 /  26    38 /  31    52 / -
@@ -506,16 +532,15 @@ static int mm_rows_launch(const MmArgs &a, const char *who, int rm = 16, int rn 
 // 19.5, 16.3 with 8 rows of B, 13.3 with 8 of each; more than 256 tiles lose again (4 and 8 rows: 21).
 struct MmCost {
     int rows, columns;
-    bool one_per_cu;      // a CU holds one workgroup: what fills the card comes in whole rounds of 256
     double alone, full;
 };
 constexpr MmCost kMmCosts[2][6] = {
     // E2M1 x E2M1
-    {{256, 256, true, 0.97, 1.07}, {128, 128, false, 0.50, 0.364}, {64, 128, false, 0.34, 0.253}, {64, 64, false, 0.27, 0.173},
-     {16, 64, false, 0.20, 0.18}, {16, 32, false, 0.11, 0.105}},
+    {{256, 256, 0.92, 1.07}, {128, 128, 0.50, 0.364}, {64, 128, 0.34, 0.253}, {64, 64, 0.27, 0.173},
+     {16, 64, 0.20, 0.18}, {16, 32, 0.11, 0.105}},
     // E4M3 x E2M1
-    {{256, 256, true, 2.55, 2.74}, {128, 128, false, 1.15, 0.88}, {64, 128, false, 0.62, 0.469}, {64, 64, false, 0.45, 0.261},
-     {16, 64, false, 0.25, 0.22}, {16, 32, false, 0.15, 0.14}},
+    {{256, 256, 2.1, 2.46}, {128, 128, 1.15, 0.88}, {64, 128, 0.62, 0.469}, {64, 64, 0.45, 0.261},
+     {16, 64, 0.25, 0.22}, {16, 32, 0.15, 0.14}},
 };
 
 struct MmPlan {
@@ -527,18 +552,18 @@ static MmPlan mm_plan(const MmArgs &a, bool fp8)
     const auto pieces = [&](int rm, int rn) {
         return (fp8 ? 9 : 5) * (int)std::min<int64_t>(rm, a.M) + 5 * (int)std::min<int64_t>(rn, a.N);
     };
+    const auto rounds = [](double tiles) { return ceil(tiles / 256.0); };
     const auto tiles = [&](int rm, int rn) { return (double)ceil_div(a.M, rm) * (double)ceil_div(a.N, rn); };
     for (int rm = 16; rm >= 4; rm /= 2)
         for (int rn = 16; rn >= 4; rn /= 2)
             if (tiles(rm, rn) <= 256.0 && pieces(rm, rn) < pieces(plan.rm, plan.rn)) plan = {6, rm, rn};
     const double touched = 0.00032 * pieces(plan.rm, plan.rn);
-    double least = std::max(0.02 + touched, (0.04 + touched) * (tiles(plan.rm, plan.rn) / 256.0));
+    const double last = rounds(tiles(plan.rm, plan.rn));
+    double least = last > 1.0 ? (0.04 + touched) * last : 0.02 + touched;
     for (int v = 0; v < 6; v++) {
         if (v < 4 && a.steps >= 65536) continue;                 // longer rows than the tiles' offsets reach
         const MmCost &c = kMmCosts[fp8][v];
-        double rounds = (double)ceil_div(a.M, c.rows) * (double)ceil_div(a.N, c.columns) / 256.0;
-        if (c.one_per_cu) rounds = ceil(rounds);
-        const double cost = std::max(c.alone, c.full * rounds);
+        const double cost = std::max(c.alone, c.full * rounds(tiles(c.rows, c.columns)));
         if (cost < least) plan.kind = v, least = cost;
     }
     return plan;
