@@ -1216,39 +1216,35 @@ static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
     //   5818 x 500 fp32       - /  29       - /  66 (256 threads), 10 x 500 12, 12
     //   5338 x 741 bf16       - /  43       - /  68 (256 threads), 10 x 1000 14, 14
     //   1024 x 2000 bf16     10 /  21      26 /  65 (1024 threads)
-    //    100 x 4000 bf16      9 /  18       9 /  21 (1024 threads)
     //    200 x 8000 bf16     10 /  25       9 /  27 (1024 threads of one group)
-    //    600 x 8000 bf16      - /  49       - /  71
     //    256 x 16000 bf16    13 /  28      18 /  37 (by chunks)
-    //     10 x 16000 fp32    12 /  29      14 /  31 (512 threads of four groups: two workgroups a CU, so for more rows than CUs)
-    //   1024 x 16000 fp32    39 /  83      50 / 115 (1024 threads of two)
-    //   1024 x 32768 bf16    82 / 113      82 / 160 (1024 threads, one workgroup a CU)
-    //    400 x 131072 bf16    - / 155       - / 161 (512 threads), 1 x 131072 fp32 16 / 37, 16 / 43
-    // By chunks also: 64 x 32768 bf16 17 / 31, 5 x 50001 fp16 17 / 32, 256 x 131072 bf16 51 / 93, the largest entry alone 20.
-    const dim3 rows((unsigned)a.R);
+    // A CU holds 1024 threads of these; where rows outnumber what all of them hold, half the threads a row (with
+    // top_p, a row's threads as they are / half of them):
+    //   8, 1024, 4000 x 2000 bf16      15, 21,  67 /  19, 22,  54
+    //   8,  512, 4000 x 4000 bf16      17, 23, 148 /  20, 24, 101
+    //   8,  512, 4000 x 8000 bf16      24, 34, 219 /  31, 36, 165
+    //  10,      1024 x 16000 fp32      29,     115 /  31,      83
+    // By chunks: 64 x 32768 bf16 17 / 31, 5 x 50001 fp16 17 / 32, 256 x 131072 bf16 51 / 93, the largest entry alone 20.  512
+    // threads a row, 1024 for the longest: 1024 x 32768 bf16 113, 160; 400 x 131072 161, 155; 1 x 131072 fp32 43, 37.
+    const auto launch = [&](auto *kernel, int threads) { kernel<<<dim3((unsigned)a.R), dim3(threads), 0, st>>>(a); };
     if (a.V <= 64) {
         sample_short_kernel<T><<<dim3((unsigned)ceil_div(a.R, 4)), dim3(256), 0, st>>>(a);
     } else if (a.V <= 64 * kGroup - 8) {                 // a row that starts inside a group reaches into one more
-        sample_row_kernel<T, 64, 1><<<rows, dim3(64), 0, st>>>(a);
+        launch(sample_row_kernel<T, 64, 1>, 64);
     } else if (a.V <= 128 * kGroup - 8) {
-        sample_row_kernel<T, 128, 1><<<rows, dim3(128), 0, st>>>(a);
+        launch(sample_row_kernel<T, 128, 1>, 128);
     } else if (a.V <= 256 * kGroup - 8) {
-        sample_row_kernel<T, 256, 1><<<rows, dim3(256), 0, st>>>(a);
+        a.R <= 1024 ? launch(sample_row_kernel<T, 256, 1>, 256) : launch(sample_row_kernel<T, 128, 2>, 128);
     } else if (a.V <= 512 * kGroup - 8) {
-        sample_row_kernel<T, 512, 1><<<rows, dim3(512), 0, st>>>(a);
+        a.R <= 512 ? launch(sample_row_kernel<T, 512, 1>, 512) : launch(sample_row_kernel<T, 256, 2>, 256);
     } else if (a.V <= 1024 * kGroup - 8) {
-        sample_row_kernel<T, 512, 2><<<rows, dim3(512), 0, st>>>(a);
-    } else if (a.V <= kTokenLocalV && a.R > 256) {
-        sample_row_kernel<T, 512, 4><<<rows, dim3(512), 0, st>>>(a);
+        a.R <= 512 ? launch(sample_row_kernel<T, 512, 2>, 512) : launch(sample_row_kernel<T, 256, 4>, 256);
     } else if (a.V <= kTokenLocalV) {
-        sample_row_kernel<T, 1024, 2><<<rows, dim3(1024), 0, st>>>(a);
+        a.R <= 256 ? launch(sample_row_kernel<T, 1024, 2>, 1024) : launch(sample_row_kernel<T, 512, 4>, 512);
     } else {
         token_chunk_kernel<T><<<dim3((unsigned)std::min<int64_t>(a.R * a.chunks, kChunkGrid)), dim3(512), 0, st>>>(a);
         if (const int rc = check_launch(who)) return rc;
-        if (a.V <= 65536)
-            sample_row_kernel<T, 512, 0><<<rows, dim3(512), 0, st>>>(a);
-        else
-            sample_row_kernel<T, 1024, 0><<<rows, dim3(1024), 0, st>>>(a);
+        a.V <= 65536 ? launch(sample_row_kernel<T, 512, 0>, 512) : launch(sample_row_kernel<T, 1024, 0>, 1024);
     }
     return check_launch(who);
 }

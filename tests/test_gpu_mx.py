@@ -732,3 +732,18 @@ def test_product_of_very_many_rows(ops, a_format):
     got = ops.mx_mm_nt(A, B, torch.bfloat16)
     assert not bool(got[:-2].any())
     assert got[-2:].tolist() == [[1.0, -2.0, 3.0]] * 2
+
+
+@pytest.mark.parametrize("R, V", [(1200, 1500), (700, 3000), (600, 6001), (300, 12001)], ids=str)
+def test_tokens_of_many_rows(ops, R, V):
+    """Rows that outnumber what the card holds at once: a few distinct ones repeated, drawn as the few are."""
+    g = torch.Generator().manual_seed(R)
+    few = torch.cat([hard_rows(V, torch.float32), torch.randn(8, V, generator=g) * 2.5])
+    at = torch.randint(0, 16, (R,), generator=g)
+    words = words_of(R, 3)
+    x = few[at].cuda()
+    for kw in HARD:
+        got = ops.sample_tokens_from_words(x, words.cuda(), **kw).cpu()
+        for lo in range(0, R, 100):                          # in pieces small enough for the other form
+            part = ops.sample_tokens_from_words(x[lo:lo + 100], words[lo:lo + 100].cuda(), **kw).cpu()
+            assert torch.equal(got[lo:lo + 100], part)
