@@ -1480,8 +1480,8 @@ def sample_tokens_from_words(logits, words, temperature=1.0, top_k=0, top_p=1.0,
 
     ``words`` [R]: uint32 (or int32 holding the same bit patterns), e.g. from :func:`philox_words`.  Every setting is a
     number for all rows or a tensor [R] (float32; ``top_k`` int32); numbers are rounded to float32 too, so that both draw the
-    same tokens.  Weights are summed as integers: the same tokens
-    on every run.  Stands beside :func:`sample_bits_from_words`, which draws bits."""
+    same tokens.  NaN in a tensor: the largest entry (``temperature``), nothing cut (``top_p``, ``min_p``).  Weights are
+    summed as integers: the same tokens on every run.  Stands beside :func:`sample_bits_from_words`, which draws bits."""
     _check(logits, "logits")
     _check(words, "words")
     _same_device(logits, words)

@@ -747,3 +747,20 @@ def test_tokens_of_many_rows(ops, R, V):
         for lo in range(0, R, 100):                          # in pieces small enough for the other form
             part = ops.sample_tokens_from_words(x[lo:lo + 100], words[lo:lo + 100].cuda(), **kw).cpu()
             assert torch.equal(got[lo:lo + 100], part)
+
+
+@pytest.mark.parametrize("V", [20, 300, 5000, 20003])
+def test_tokens_with_extreme_settings_per_row(ops, V):
+    nan, inf = float("nan"), float("inf")
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(V)).cuda() * 2
+    words = words_of(4, 1).cuda()
+    t = lambda *v: torch.tensor(v, device="cuda")
+    top = x.argmax(1).int()
+    plain = ops.sample_tokens_from_words(x, words)
+    assert torch.equal(ops.sample_tokens_from_words(x, words, top_p=t(nan, inf, 1.0, 2.0), min_p=t(nan, -1.0, -inf, 0.0)), plain)
+    assert torch.equal(ops.sample_tokens_from_words(x, words, temperature=t(nan, 0.0, -inf, -1.0)), top)
+    assert torch.equal(ops.sample_tokens_from_words(x, words, top_p=t(-1.0, -inf, 0.0, 1e-30)), top)
+    assert torch.equal(ops.sample_tokens_from_words(x, words, min_p=t(1.0, inf, 2.0, 1.0)), top)
+    k = torch.tensor([1, 0, -(2 ** 31), 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    got = ops.sample_tokens_from_words(x, words, top_k=k)
+    assert got[0] == top[0] and torch.equal(got[1:], plain[1:])
