@@ -1297,9 +1297,12 @@ class MXRows:
     ``codes`` uint8 [rows, Kp/2] ("fp4", element 2i in the low half of byte i) or [rows, Kp] ("fp8"), ``scales`` uint8
     [rows, Kp/32] (scale 2**(byte - 127), 255: the block stands for NaN).  Positions K..Kp-1 must hold zero codes, and
     blocks of such positions only no scale byte 255; :func:`mx_quantize` and :func:`rms_norm_mx` write
-    them so.  Holds the tensors it is given (both start 16 and 4 bytes aligned); nothing is laid out again."""
+    them so.  Holds the tensors it is given (both start 16 and 4 bytes aligned); nothing is laid out again.  Threads may share
+    rows as they share tensors."""
 
-    __slots__ = ("_codes", "_scales", "_code_bytes", "_device", "rows", "K", "format")
+    # _joint: rows written by a kernel hold codes and scales in one allocation, from beginning to end; None: a user's tensors.
+    # _views: (codes, scales), set in one assignment; None until somebody asks for the parts of a joint allocation.
+    __slots__ = ("_joint", "_views", "_code_bytes", "_device", "rows", "K", "format")
 
     def __init__(self, codes, scales, K, format="fp4"):
         if format not in _MX_FORMATS:
@@ -1315,7 +1318,7 @@ class MXRows:
         padded = ceil_div(K, _MX_STEP) * _MX_STEP
         assert K >= 0 and code_bytes == padded // _MX_FORMATS[format][1]
         assert tuple(scales.shape) == (rows, padded // 32)
-        self._codes, self._scales, self._code_bytes, self._device = codes, scales, code_bytes, codes.device
+        self._joint, self._views, self._code_bytes, self._device = None, (codes, scales), code_bytes, codes.device
         self.rows, self.K, self.format = rows, K, format
 
     @classmethod
@@ -1326,25 +1329,35 @@ class MXRows:
         padded = ceil_div(K, _MX_STEP) * _MX_STEP
         self = cls.__new__(cls)
         self._code_bytes = padded // _MX_FORMATS[format][1]
-        self._codes = None
-        self._scales = torch.empty(rows * (self._code_bytes + padded // 32), dtype=torch.uint8, device=device)
+        self._joint = torch.empty(rows * (self._code_bytes + padded // 32), dtype=torch.uint8, device=device)
+        self._views = None
         self._device = device
         self.rows, self.K, self.format = rows, K, format
         return self
 
     def _pointers(self):
-        if self._codes is None:
-            both = self._scales.data_ptr()
+        if self._joint is not None:
+            both = self._joint.data_ptr()
             return both, both + self.rows * self._code_bytes
-        return self._codes.data_ptr(), self._scales.data_ptr()
+        codes, scales = self._views
+        return codes.data_ptr(), scales.data_ptr()
 
     def _parts(self):
-        if self._codes is None:
-            both, rows, n = self._scales, self.rows, self._code_bytes
+        views = self._views
+        if views is None:
+            joint, rows, n = self._joint, self.rows, self._code_bytes
             per_row = ceil_div(self.K, _MX_STEP) * (_MX_STEP // 32)
-            self._codes = both.as_strided((rows, n), (n, 1))
-            self._scales = both.as_strided((rows, per_row), (per_row, 1), rows * n)
-        return self._codes, self._scales
+            views = self._views = (joint.as_strided((rows, n), (n, 1)),
+                                   joint.as_strided((rows, per_row), (per_row, 1), rows * n))
+        return views
+
+    def __getstate__(self):
+        # views of a joint allocation are made again: pickled next to it they would come back as memory of their own
+        return (self._joint, self._views if self._joint is None else None, self._code_bytes, self.rows, self.K, self.format)
+
+    def __setstate__(self, state):
+        self._joint, self._views, self._code_bytes, self.rows, self.K, self.format = state
+        self._device = (self._views[0] if self._joint is None else self._joint).device
 
     @property
     def codes(self):

@@ -1,8 +1,12 @@
 """Microscaled rows, norm, product and token sampler without a GPU: the oracle's own pins, and what is refused before
 anything is launched."""
+import copy
 import ctypes
 import math
 import os
+import pickle
+import sys
+import threading
 
 import numpy as np
 import pytest
@@ -122,3 +126,90 @@ def test_python_refuses_host_tensors():
         ops.MXRows(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(2, 4, dtype=torch.uint8), 64)
     with pytest.raises(ValueError, match="format"):
         ops.MXRows(x, x, 64, "fp6")
+
+
+# ---- rows that a kernel wrote, taken apart while another thread uses them ----------------------------------------------
+def _before_line(n, call, other):
+    """Runs ``call``, and ``other`` before the n-th line that it runs in the rows' own code, as a thread that takes its turn there
+    would.  -> (what call gave, what other gave in a list, empty where there are fewer lines)"""
+    from nesgpu_amd.extensions import booleanOperations as ops
+    left, got = [n], []
+
+    def trace(frame, event, arg):
+        if frame.f_code.co_filename != ops.__file__:
+            return None
+        if event == "line":
+            left[0] -= 1
+            if left[0] == -1:
+                got.append(other())                          # not traced: the tracer is off inside itself
+        return trace
+
+    before = sys.gettrace()
+    sys.settrace(trace)
+    try:
+        return call(), got
+    finally:
+        sys.settrace(before)
+
+
+@pytest.mark.parametrize("format", O.FORMATS)
+@pytest.mark.parametrize("call", ["pointers", "codes", "scales"])
+@pytest.mark.parametrize("other", ["pointers", "codes", "scales"])
+def test_rows_are_taken_apart_between_any_two_lines_of_their_use(format, call, other):
+    from nesgpu_amd.extensions import booleanOperations as ops
+    rows, K = 5, 200
+    n = 256 if format == "fp8" else 128
+    for line in range(100):
+        q = ops.MXRows._empty(rows, K, format, "cpu")
+        use = {"pointers": q._pointers, "codes": lambda: q.codes, "scales": lambda: q.scales}
+        codes = q._pointers()[0]
+        scales = codes + rows * n
+
+        def right(which, got):
+            if which == "pointers":
+                return tuple(got) == (codes, scales)
+            if which == "codes":
+                return (got.data_ptr(), tuple(got.shape), got.stride()) == (codes, (rows, n), (n, 1))
+            return (got.data_ptr(), tuple(got.shape), got.stride()) == (scales, (rows, 8), (8, 1))
+
+        mine, theirs = _before_line(line, use[call], use[other])
+        assert right(call, mine) and all(right(other, t) for t in theirs), line
+        assert all(right(which, use[which]()) for which in use), line
+        if not theirs:
+            break
+    assert line > 2 and not theirs
+
+
+def test_rows_are_used_by_two_threads():
+    from nesgpu_amd.extensions import booleanOperations as ops
+    rows, K = 3, 130
+    before, turns, wrong = sys.getswitchinterval(), 2000, []
+    sys.setswitchinterval(1e-6)
+    try:
+        for _ in range(turns):
+            q = ops.MXRows._empty(rows, K, "fp8", "cpu")
+            start = q._pointers()[0]
+            other = threading.Thread(target=lambda: (q.scales, q.codes))
+            other.start()
+            for _ in range(20):
+                if q._pointers() != (start, start + rows * 256) or q.scales.data_ptr() != start + rows * 256:
+                    wrong.append(q)
+            other.join()
+    finally:
+        sys.setswitchinterval(before)
+    assert not wrong
+
+
+def test_copies_of_rows_keep_their_parts_in_one_place():
+    """What is written through a copy's codes is what the kernels read there, whether the parts were made before or not."""
+    from nesgpu_amd.extensions import booleanOperations as ops
+    for made in (False, True):
+        q = ops.MXRows._empty(4, 40, "fp4", torch.device("cpu"))
+        q._joint.copy_(torch.arange(q._joint.numel()) % 251)
+        if made:
+            q.codes
+        for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+            assert other._pointers() == (other.codes.data_ptr(), other.scales.data_ptr())
+            assert torch.equal(other.codes, q.codes) and torch.equal(other.scales, q.scales)
+            assert (other.rows, other.K, other.format, other.device) == (q.rows, q.K, q.format, q.device)
+        assert copy.copy(q)._pointers() == q._pointers()
