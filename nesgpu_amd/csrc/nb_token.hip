@@ -1207,6 +1207,12 @@ __global__ __launch_bounds__(THREADS, 4) void sample_row_kernel(TokenArgs a)
 }
 
 static int token_chunks(int64_t V) { return (int)ceil_div(V + kGroup - 1, kChunkGroups * kGroup); }
+// Rows of one launch, more of them in launches that follow each other: a grid's threads are counted in 32 bits, and the
+// chunks' records of a launch are kept below 6.5 GB (the next launch takes the same memory).
+static int64_t token_rows(int64_t V)
+{
+    return V <= 64 ? 1LL << 24 : V <= kTokenLocalV ? 1LL << 21 : (1LL << 21) / token_chunks(V);
+}
 
 template <typename T>
 static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
@@ -1254,8 +1260,8 @@ static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
 extern "C" {
 int64_t nb_sample_tokens_workspace_bytes(int64_t R, int64_t V)
 {
-    if (R <= 0 || V <= nb::kTokenLocalV || V > nb::kTokenMaxV || R >= (1LL << 22)) return 0;
-    return R * nb::token_chunks(V) * (int64_t)sizeof(nb::TokenChunk);
+    if (R <= 0 || V <= nb::kTokenLocalV || V > nb::kTokenMaxV) return 0;
+    return std::min(R, nb::token_rows(V)) * nb::token_chunks(V) * (int64_t)sizeof(nb::TokenChunk);
 }
 
 int nb_sample_tokens(int32_t *out, const void *logits, int type, const uint32_t *words, const float *temperature,
@@ -1266,7 +1272,7 @@ int nb_sample_tokens(int32_t *out, const void *logits, int type, const uint32_t 
     const char *who = "nb_sample_tokens";
     NB_REQUIRE(R >= 0 && V >= 1, "%s: bad shape", who);
     NB_REQUIRE(V <= nb::kTokenMaxV, "%s: rows of %lld entries, at most %lld", who, (long long)V, (long long)nb::kTokenMaxV);
-    NB_REQUIRE(R < (1LL << 22) && R * V < (1LL << 34), "%s: too many rows", who);
+    NB_REQUIRE(R <= (1LL << 40), "%s: too many rows", who);
     NB_REQUIRE(type >= NB_TYPE_F32 && type <= NB_TYPE_I32, "%s: type %d", who, type);
     NB_REQUIRE(temperature || temperature_all == temperature_all, "%s: temperature is NaN", who);
     NB_REQUIRE(top_p || top_p_all == top_p_all, "%s: top_p is NaN", who);
@@ -1291,12 +1297,20 @@ int nb_sample_tokens(int32_t *out, const void *logits, int type, const uint32_t 
     }
     int log2v = 0;
     while ((1LL << log2v) < V) log2v++;
-    const nb::TokenArgs a{out, logits, words, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all,
-                          top_k_all, R, (int)V, std::min(51, 61 - log2v), nb::token_chunks(V), (uint8_t *)workspace};
+    const int64_t most = nb::token_rows(V), size = type == NB_TYPE_F32 || type == NB_TYPE_I32 ? 4 : 2;
     const hipStream_t st = nb::as_stream(stream);
-    if (type == NB_TYPE_F32) return nb::token_launch<float>(a, st, who);
-    if (type == NB_TYPE_F16) return nb::token_launch<_Float16>(a, st, who);
-    if (type == NB_TYPE_BF16) return nb::token_launch<nb::Bf16>(a, st, who);
-    return nb::token_launch<int32_t>(a, st, who);
+    for (int64_t r0 = 0; r0 < R; r0 += most) {
+        const auto from = [&](auto *settings) { return settings ? settings + r0 : nullptr; };
+        const nb::TokenArgs a{out + r0, (const uint8_t *)logits + r0 * V * size, words + r0, from(temperature), from(top_p),
+                              from(min_p), from(top_k), temperature_all, top_p_all, min_p_all, top_k_all,
+                              std::min(most, R - r0), (int)V, std::min(51, 61 - log2v), nb::token_chunks(V),
+                              (uint8_t *)workspace};
+        const int rc = type == NB_TYPE_F32   ? nb::token_launch<float>(a, st, who)
+                       : type == NB_TYPE_F16 ? nb::token_launch<_Float16>(a, st, who)
+                       : type == NB_TYPE_BF16 ? nb::token_launch<nb::Bf16>(a, st, who)
+                                              : nb::token_launch<int32_t>(a, st, who);
+        if (rc) return rc;
+    }
+    return NB_OK;
 }
 }  // extern "C"

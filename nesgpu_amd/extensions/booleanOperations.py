@@ -1482,8 +1482,8 @@ def _row_setting(value, name, dtype, R, device):
 
 
 def sample_tokens_from_words(logits, words, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """One token (class) per row of ``logits`` [R, V] (float32, float16, bfloat16, or int32: a last layer's
-    activations) from one random word per row: int32 [R], -1 where nothing can be drawn.
+    """One token (class) per row of ``logits`` [R, V] (float32, float16, bfloat16, or int32: a last layer's activations;
+    at most 2**20 entries a row) from one random word per row: int32 [R], -1 where nothing can be drawn.
 
     A row's weights are w_i = exp((x_i - max) / temperature); NaN and -inf entries are never drawn.  The entries in
     descending order (equal ones by index) are cut to the shortest of three prefixes: the first ``top_k`` (all if

@@ -764,3 +764,25 @@ def test_tokens_with_extreme_settings_per_row(ops, V):
     k = torch.tensor([1, 0, -(2 ** 31), 2 ** 31 - 1], dtype=torch.int32, device="cuda")
     got = ops.sample_tokens_from_words(x, words, top_k=k)
     assert got[0] == top[0] and torch.equal(got[1:], plain[1:])
+
+
+# rows of more than one launch: 2^24 of at most 64 entries, 2^21 of up to 16376, 2^21 / 3 of 16385 (more than 2^34 entries)
+@pytest.mark.parametrize("R, V, dtype", [((1 << 24) + 5, 10, torch.int32), ((1 << 21) + 3, 70, torch.float16),
+                                         (1_050_000, 16385, torch.bfloat16)], ids=str)
+def test_tokens_of_rows_beyond_one_launch(ops, R, V, dtype):
+    """Every row is one of 32 under one of 32 words and one of 32 settings: all equal the table of those, and the table the oracle."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    few = torch.randn(32, V, generator=g, device="cuda") * 2.5
+    few = (few * 3).round().int() if dtype == torch.int32 else few.to(dtype)
+    words = torch.randint(-2 ** 31, 2 ** 31, (32,), generator=g, device="cuda").int()
+    settings = dict(temperature=0.5 + torch.rand(32, generator=g, device="cuda"), top_p=torch.rand(32, generator=g, device="cuda"),
+                    min_p=0.1 * torch.rand(32, generator=g, device="cuda"),
+                    top_k=torch.randint(0, 40, (32,), generator=g, device="cuda").int())
+    a, b, c = (i.reshape(-1) for i in torch.meshgrid(*[torch.arange(32, device="cuda")] * 3, indexing="ij"))
+    table = ops.sample_tokens_from_words(few[a], words[b], **{k: v[c] for k, v in settings.items()})
+    for i in torch.randint(0, 32 ** 3, (40,), generator=g, device="cuda").tolist():
+        want = O.sample(host(few[a[i]]), int(words[b[i]]) & 0xFFFFFFFF, **{k: v[c[i]].item() for k, v in settings.items()})
+        assert int(table[i]) == want
+    a, b, c = (torch.randint(0, 32, (R,), generator=g, device="cuda") for _ in range(3))
+    got = ops.sample_tokens_from_words(few[a], words[b], **{k: v[c] for k, v in settings.items()})
+    assert torch.equal(got, table[(a * 32 + b) * 32 + c])

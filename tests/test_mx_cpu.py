@@ -213,3 +213,19 @@ def test_copies_of_rows_keep_their_parts_in_one_place():
             assert torch.equal(other.codes, q.codes) and torch.equal(other.scales, q.scales)
             assert (other.rows, other.K, other.format, other.device) == (q.rows, q.K, q.format, q.device)
         assert copy.copy(q)._pointers() == q._pointers()
+
+
+# ---- rows of logits beyond one launch -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("R, V", [(1 << 22, 10), (4096 * 1024, 10), ((1 << 22) + 3, 1000), (1 << 30, 64), (1 << 20, 1 << 14),
+                                  (1 << 22, 20000), (1 << 20, 1 << 20)])
+def test_any_number_of_rows_of_logits_is_taken(lib, R, V):
+    """The rows' number is looked at before the pointers: what stops these calls is the missing logits (status 1), not a
+    shape (2)."""
+    one = ctypes.c_void_p(256)
+    args = (None, 1.0, None, 0, None, 1.0, None, 0.0)
+    assert lib.nb_sample_tokens(one, None, 0, one, *args, R, V, None, 0, None) == 1
+    work = lib.nb_sample_tokens_workspace_bytes(R, V)
+    assert (work > 0) == (V > 16376) and work < 13 << 29          # 6.5 GiB
+    if work:                                                      # and a short one is refused
+        assert lib.nb_sample_tokens(one, one, 0, one, *args, R, V, one, work - 1, None) == 2
+    assert lib.nb_sample_tokens(one, None, 0, one, *args, (1 << 40) + 1, V, None, 0, None) == 2
