@@ -546,9 +546,12 @@ int nb_rms_norm_mx(uint8_t *codes, uint8_t *scales, void *residual_out, const vo
                    int residual_type, const void *weight, int weight_type, double eps, int format, int64_t rows,
                    int64_t K, nb_stream_t stream);
 /* nb_mx_mm_nt: C[m, n] = sum_k A[m, k] * B[n, k] over MX rows, A in either format, B in E2M1; fp32 sums, rounded once to
- * C's type (fp32, fp16, bf16); C [M, N]. */
+ * C's type (fp32, fp16, bf16); C [M, N].  M, N, K <= 2^30. */
 int nb_mx_mm_nt(void *C, int type, const uint8_t *A, const uint8_t *A_scales, int A_format, const uint8_t *B,
                 const uint8_t *B_scales, int64_t M, int64_t N, int64_t K, nb_stream_t stream);
+/* nb_mx_mm_tile: the tile of outputs, rows * 65536 + columns, that a workgroup of nb_mx_mm_nt makes for these sizes (from the
+ * sizes alone, on the host; another tile is another kernel); 0 where the sizes or the format are refused. */
+int64_t nb_mx_mm_tile(int64_t M, int64_t N, int64_t K, int A_format);
 
 /* ---- tokens from logits and supplied words --------------------------------------------------------------------------
  * nb_sample_tokens: one token per row of logits [R, V] (fp32, fp16, bf16 or int32), out int32 [R].  Per row, with T the

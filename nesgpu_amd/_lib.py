@@ -96,6 +96,7 @@ _SIZES = {
     "nb_flip_layer_table_words": [],
     "nb_law_workspace_bytes": [],
     "nb_sample_tokens_workspace_bytes": [_I64, _I64],
+    "nb_mx_mm_tile": [_I64, _I64, _I64, _I32],
 }
 
 

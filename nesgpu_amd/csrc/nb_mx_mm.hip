@@ -544,27 +544,32 @@ constexpr MmCost kMmCosts[2][6] = {
 };
 
 struct MmPlan {
-    int kind, rm, rn;     // rm, rn: rows of A and B in a tile of the last kind
+    int kind, rm, rn;     // rm, rn: rows of A and B in a tile
 };
-static MmPlan mm_plan(const MmArgs &a, bool fp8)
+// Tiles of one launch: its threads are counted in 32 bits, by kinds of 8 waves (the first, the last) and of 4.
+constexpr double kMmMost[7] = {1 << 22, 1 << 23, 1 << 23, 1 << 23, (1 << 24) - 1, (1 << 24) - 1, (1 << 23) - 1};
+
+static MmPlan mm_plan(int64_t M, int64_t N, int64_t steps, bool fp8)
 {
     MmPlan plan{6, 16, 16};
     const auto pieces = [&](int rm, int rn) {
-        return (fp8 ? 9 : 5) * (int)std::min<int64_t>(rm, a.M) + 5 * (int)std::min<int64_t>(rn, a.N);
+        return (fp8 ? 9 : 5) * (int)std::min<int64_t>(rm, M) + 5 * (int)std::min<int64_t>(rn, N);
     };
     const auto rounds = [](double tiles) { return ceil(tiles / 256.0); };
-    const auto tiles = [&](int rm, int rn) { return (double)ceil_div(a.M, rm) * (double)ceil_div(a.N, rn); };
+    const auto tiles = [&](int rm, int rn) { return (double)ceil_div(M, rm) * (double)ceil_div(N, rn); };
     for (int rm = 16; rm >= 4; rm /= 2)
         for (int rn = 16; rn >= 4; rn /= 2)
             if (tiles(rm, rn) <= 256.0 && pieces(rm, rn) < pieces(plan.rm, plan.rn)) plan = {6, rm, rn};
     const double touched = 0.00032 * pieces(plan.rm, plan.rn);
     const double last = rounds(tiles(plan.rm, plan.rn));
     double least = last > 1.0 ? (0.04 + touched) * last : 0.02 + touched;
+    if (tiles(plan.rm, plan.rn) > kMmMost[6]) least = INFINITY;
     for (int v = 0; v < 6; v++) {
-        if (v < 4 && a.steps >= 65536) continue;                 // longer rows than the tiles' offsets reach
+        if (v < 4 && steps >= 65536) continue;                   // longer rows than the tiles' offsets reach
         const MmCost &c = kMmCosts[fp8][v];
+        if (tiles(c.rows, c.columns) > kMmMost[v]) continue;
         const double cost = std::max(c.alone, c.full * rounds(tiles(c.rows, c.columns)));
-        if (cost < least) plan.kind = v, least = cost;
+        if (cost < least) plan = {v, c.rows, c.columns}, least = cost;
     }
     return plan;
 }
@@ -572,7 +577,7 @@ static MmPlan mm_plan(const MmArgs &a, bool fp8)
 template <bool FP8, typename O>
 static int mm_launch(const MmArgs &a, const char *who)
 {
-    const MmPlan plan = mm_plan(a, FP8);
+    const MmPlan plan = mm_plan(a.M, a.N, a.steps, FP8);
     switch (plan.kind) {
         case 0: return mm_tile_launch<FP8, O, 4, 2, 4, 8, FP8 ? 1 : 2, FP8 ? 3 : 2>(a, who);
         case 1: return mm_tile_launch<FP8, O, 2, 2, 4, 4, 1, 3>(a, who);
@@ -587,6 +592,16 @@ static int mm_launch(const MmArgs &a, const char *who)
 }  // namespace nb
 
 extern "C" {
+int64_t nb_mx_mm_tile(int64_t M, int64_t N, int64_t K, int A_format)
+{
+    if (M < 1 || N < 1 || K < 1 || M > (1LL << 30) || N > (1LL << 30) || K > (1LL << 30) ||
+        (A_format != NB_MX_FP4 && A_format != NB_MX_FP8))
+        return 0;
+    const nb::MmPlan plan = nb::mm_plan(M, N, nb::mx_padded(K) / nb::kMxStep, A_format == NB_MX_FP8);
+    if ((double)nb::ceil_div(M, plan.rm) * (double)nb::ceil_div(N, plan.rn) > nb::kMmMost[plan.kind]) return 0;
+    return (int64_t)plan.rm << 16 | plan.rn;
+}
+
 int nb_mx_mm_nt(void *C, int type, const uint8_t *A, const uint8_t *A_scales, int A_format, const uint8_t *B,
                 const uint8_t *B_scales, int64_t M, int64_t N, int64_t K, nb_stream_t stream)
 {

@@ -786,3 +786,19 @@ def test_tokens_of_rows_beyond_one_launch(ops, R, V, dtype):
     a, b, c = (torch.randint(0, 32, (R,), generator=g, device="cuda") for _ in range(3))
     got = ops.sample_tokens_from_words(few[a], words[b], **{k: v[c] for k, v in settings.items()})
     assert torch.equal(got, table[(a * 32 + b) * 32 + c])
+
+
+@pytest.mark.parametrize("N", [1, 3])
+def test_product_of_more_rows_than_a_launch_of_square_tiles_holds(ops, N):
+    """More than 2^23 tiles of 64 x 64."""
+    M, K = (1 << 29) + 70, 1
+    A = ops.MXRows(torch.zeros(M, 64, dtype=torch.uint8, device="cuda"),
+                   torch.full((M, 4), 127, dtype=torch.uint8, device="cuda"), K, "fp4")
+    A.codes[-2:, 0] = 0x02
+    A.codes[1 << 28, 0] = 0x02
+    B = ops.mx_quantize(torch.tensor([[1.0], [-2.0], [3.0]], device="cuda")[:N].contiguous(), "fp4")
+    got = ops.mx_mm_nt(A, B, torch.bfloat16)
+    for at in (M - 2, M - 1, 1 << 28):
+        assert got[at].tolist() == [1.0, -2.0, 3.0][:N]
+        got[at] = 0
+    assert not bool(got.any())

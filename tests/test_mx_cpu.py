@@ -229,3 +229,28 @@ def test_any_number_of_rows_of_logits_is_taken(lib, R, V):
     if work:                                                      # and a short one is refused
         assert lib.nb_sample_tokens(one, one, 0, one, *args, R, V, one, work - 1, None) == 2
     assert lib.nb_sample_tokens(one, None, 0, one, *args, (1 << 40) + 1, V, None, 0, None) == 2
+
+
+# ---- the product's tiles --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("format", [0, 1])
+def test_every_size_has_a_tile_that_one_launch_holds(lib, format):
+    """All sizes up to 2^30 whose output of two bytes each fits 288 GB; a launch has threads for 2^22 tiles of 256 x 256 or 2^23 of others, and
+    2^23 - 1 or 2^24 - 1 of the narrow ones."""
+    most = {(256, 256): 1 << 22, (128, 128): 1 << 23, (64, 128): 1 << 23, (64, 64): 1 << 23, (16, 64): (1 << 24) - 1,
+            (16, 32): (1 << 24) - 1}
+    sizes = sorted({min(int(2 ** (e / 2)) + d, 1 << 30) for e in range(61) for d in (0, 1)})
+    for M in sizes:
+        for N in sizes:
+            if M * N > 1 << 37:
+                continue
+            for K in (1, 700, 65535 * 128, 65536 * 128):
+                if K > 700 and M + N > 1 << 17:
+                    continue
+                t = lib.nb_mx_mm_tile(M, N, K, format)
+                rows, columns = t >> 16, t & 0xFFFF
+                assert rows and columns, (M, N, K)
+                tiles = -(-M // rows) * -(-N // columns)
+                assert tiles <= most.get((rows, columns), (1 << 23) - 1), (M, N, K, rows, columns)
+    for bad in ((0, 1, 1), (1, 1, 0), (1, -1, 1), ((1 << 30) + 1, 1, 1), (1, 1, (1 << 30) + 1)):
+        assert lib.nb_mx_mm_tile(*bad, format) == 0
+    assert lib.nb_mx_mm_tile(1, 1, 1, 2) == 0
