@@ -802,3 +802,59 @@ def test_product_of_more_rows_than_a_launch_of_square_tiles_holds(ops, N):
         assert got[at].tolist() == [1.0, -2.0, 3.0][:N]
         got[at] = 0
     assert not bool(got.any())
+
+
+# ---- every kernel of the product and of the sampler ----------------------------------------------------------------------
+# sizes by the tile that they take; the test asks the library whether they still do
+TILES = {
+    "fp8": {(256, 256): [(4001, 8190)], (128, 128): [(2047, 4095), (2000, 4000)], (64, 128): [(3000, 3000), (4137, 745)],
+            (64, 64): [(2049, 2100), (1596, 436)], (16, 64): [(939, 164), (64, 7132)], (16, 32): [(645, 179), (300, 1100)],
+            (16, 16): [(2489, 35), (1, 3786)], (8, 16): [(101, 163), (27, 983)], (16, 4): [(1, 671)], (4, 4): [(39, 36)]},
+    "fp4": {(256, 256): [(4001, 8190)], (128, 128): [(3001, 2501), (2047, 4095)], (64, 128): [(273, 3825), (1023, 1025)],
+            (64, 64): [(588, 1432), (300, 1100)], (16, 64): [(70, 2000), (344, 407)], (16, 32): [(794, 97), (33, 1900)],
+            (16, 16): [(127, 275)], (8, 8): [(276, 35)], (16, 8): [(27, 983)], (4, 4): [(30, 18)]},
+}
+
+
+@pytest.mark.parametrize("K, moved", [(512, False), (1024, True), (1104, False)], ids=["512", "1024-scales-on-4-bytes", "1104"])
+@pytest.mark.parametrize("a_format, tile, shape", [(f, t, s) for f, v in TILES.items() for t, shapes in v.items() for s in shapes],
+                         ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else v)
+def test_every_tile_makes_exact_sums(ops, a_format, tile, shape, K, moved):
+    """E4M3: of every eight neighbours two large values that cancel and two that are 17 binades smaller; E2M1: small whole numbers.
+    Blocks and rows have scales of their own.  With blocks 2^0 to 2^4 apart the running sum is a multiple of 2^-10 below 2^13, 23 bits
+    times the two rows' scales: exact in fp32, and what is stored is that sum rounded once.  The fp16 product is first called inside a
+    captured graph, and replayed with the signs of A's codes turned."""
+    from nesgpu_amd import _lib
+    M, N = shape
+    taken = _lib.load().nb_mx_mm_tile(M, N, K, O.FORMATS.index(a_format))
+    assert (taken >> 16, taken & 0xFFFF) == tile
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    power = lambda lo, hi, *size: torch.exp2(torch.randint(lo, hi + 1, size, generator=g, device="cuda").float())
+    whole = lambda lo, hi, *size: torch.randint(lo, hi + 1, size, generator=g, device="cuda").float()
+    if a_format == "fp8":
+        a, b = torch.zeros(M, K, device="cuda"), torch.ones(N, K, device="cuda")
+        a[:, 0::8], a[:, 1::8] = 256.0, -256.0
+        a[:, 2::8], a[:, 5::8] = whole(1, 7, M, K // 8) / 512, whole(8, 15, M, K // 8) / 512
+        b[:, 2::8] = torch.tensor([0.5, 1.5, -3.0], device="cuda")[whole(0, 2, N, K // 8).long()]
+    else:
+        a, b = whole(-3, 3, M, K), whole(-2, 2, N, K)
+    blocks = -(-K // 32)
+    a *= power(0, 3, M, blocks).repeat_interleave(32, 1)[:, :K] * power(-6, 6, M, 1)
+    b *= power(0, 1, N, blocks).repeat_interleave(32, 1)[:, :K] * power(-3, 3, N, 1)
+    A, B = ops.mx_quantize(a, a_format), ops.mx_quantize(b, "fp4")
+    assert torch.equal(ops.mx_dequantize(A, torch.float32), a) and torch.equal(ops.mx_dequantize(B, torch.float32), b)
+    if moved:
+        flat = torch.zeros(A.scales.numel() + 16, dtype=torch.uint8, device="cuda")
+        flat[4:4 + A.scales.numel()] = A.scales.view(-1)
+        A = ops.MXRows(A.codes, flat[4:4 + A.scales.numel()].view(A.scales.shape), K, a_format)
+    want = (a.double() @ b.double().t()).float()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.mx_mm_nt(A, B, torch.float16)
+    for sign in (1, -1, 1):
+        graph.replay()
+        assert torch.equal(out, (sign * want).half())
+        A.codes.bitwise_xor_(0x80 if a_format == "fp8" else 0x88)
+    A.codes.bitwise_xor_(0x80 if a_format == "fp8" else 0x88)
+    assert torch.equal(ops.mx_mm_nt(A, B), want)
+    assert torch.equal(ops.mx_mm_nt(A, B, torch.bfloat16), want.bfloat16())
