@@ -858,3 +858,33 @@ def test_every_tile_makes_exact_sums(ops, a_format, tile, shape, K, moved):
     A.codes.bitwise_xor_(0x80 if a_format == "fp8" else 0x88)
     assert torch.equal(ops.mx_mm_nt(A, B), want)
     assert torch.equal(ops.mx_mm_nt(A, B, torch.bfloat16), want.bfloat16())
+
+
+# rows that outnumber what the card holds at once, by the four forms that such rows take; the last entries of each form too
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int32], ids=IDS + ["i32"])
+@pytest.mark.parametrize("R, V", [(1100, 1017), (1100, 2040), (600, 2041), (600, 4088), (600, 4089), (600, 8184), (300, 8185),
+                                  (300, 16376)], ids=str)
+def test_tokens_of_many_rows_of_every_type(ops, R, V, dtype):
+    """Twelve rows under four words, each as often as it comes: alike wherever they stand, in storage that starts inside a load, and
+    those looked at equal to the oracle."""
+    g = torch.Generator().manual_seed(R + V)
+    few = torch.randn(4, V, generator=g) * 2.5
+    few = torch.cat([hard_rows(V, dtype), ((few * 3).round().int() if dtype == torch.int32 else few.to(dtype))])
+    few[1, -1] = few[1, 0] = few[1].max()                    # the largest entry at both ends
+    four = torch.tensor([0, -1, 123456789, -1234567890], dtype=torch.int32)
+    row, word = torch.randint(0, 12, (R,), generator=g), torch.randint(0, 4, (R,), generator=g)
+    flat = torch.empty(R * V + 1, dtype=dtype, device="cuda")
+    x = flat[1:].view(R, V)
+    x.copy_(few.cuda()[row.cuda()])
+    words = four[word].cuda()
+    pair = row * 4 + word
+    first = torch.full((48,), -1)
+    for i in range(R - 1, -1, -1):
+        first[pair[i]] = i
+    assert int(first.min()) >= 0
+    for n, kw in enumerate(HARD + [dict(temperature=0.0)]):
+        got = ops.sample_tokens_from_words(x, words, **kw).cpu()
+        assert torch.equal(got, got[first[pair]])
+        for p in ((5 * n + 7 * k) % 48 for k in range(3 if V > 5000 else 8)):
+            want = O.sample(host(few[p // 4]), int(four[p % 4]) & 0xFFFFFFFF, **kw)
+            assert int(got[first[p]]) == want, (n, p)
