@@ -194,10 +194,13 @@ __device__ __forceinline__ double row_sum(double s, double *part)
 //
 // Bound by memory: with a residual in bf16 7 + 1/32 bytes an element, 8192 x 8192 in 92 to 102 us (4.6 to 5.1 TB/s; a large
 // copy 5.1).  The weights are loaded after the sum: taken before it they cost 16 registers per piece over the barrier and a
-// third of the waves (151 us).  Without a residual the 64-bit products show: 58 us for 3.0 bytes an element, 3.5 TB/s.
+// third of the waves (151 us).  Without a residual the 64-bit products and their conversions show: 8192 x 8192 bf16, 3.0 bytes
+// an element, 58 to 60 us (3.4 TB/s) over one set of rows, 70 over three in turn; fp32, 5.0 bytes, 79 us (4.3).  Int32 sums
+// with an fp16 stream, 4096 x 1024: 8 us out of the caches, 10 to 11 over many sets (3.5 TB/s).
 // A wave per row, without barriers, up to 1024 elements: 32768 x 1024 bf16 41 us, 15530 x 547 23 us; a workgroup of 256
 // threads 52 and 34, of 128 43 and 24; four pieces a lane, up to 2048: 20000 x 1500 fp32 95 us, 79 with 256 threads.
-// One piece per thread: 8 waves a SIMD (64 registers) 16384 x 4096 90 us, 95 with 68 registers; two pieces need their 92.
+// One piece per thread: 8 waves a SIMD (64 registers) 16384 x 4096 90 us, 95 with 68 registers; two pieces need their 92.  (int32
+// with a 16-bit residual and 512 threads: two of the 64 spill.)
 // Rows above 8192 are read twice: 4096 x 16384 bf16 105 us (held by 1024 threads of two pieces 107), 2000 x 32000 fp16
 // 107 us (of four pieces 131), 3355 x 20001 fp32 215 us (219).
 template <typename X, typename R, bool FP8, bool VEC, int T, int N>

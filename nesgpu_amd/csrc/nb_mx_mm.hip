@@ -182,9 +182,10 @@ __global__ __launch_bounds__(64 * W) void mx_mm_rows_kernel(O *__restrict__ C, c
 // 16 bytes per row.
 //
 // What bounds it.  E2M1: the way from the second cache into LDS.  A tile of 256 x 256 takes 32 KB a step, of 128 x 128 16 KB,
-// and either arrives at 15 to 16 bytes a cycle and CU, however many stages are ahead (2, 3, 4 of 16 KB and 32 KB alike) and
-// however many CUs are at work (64, 256): 1.0 and 0.5 us a step, where the matrix instructions alone would take 0.45 and
-// 0.11.  8192 x 8192 x 8192 4.0 PFLOP/s.  E4M3: the matrix instructions, of which the split makes two, at 70 to 80 % of their rate.
+// and either arrives at 13 to 16 bytes a cycle and CU, however many stages are ahead (2, 3, 4 of 16 KB and 32 KB alike) and
+// nearly however many CUs are at work (64, 256): 1.0 to 1.2 and 0.5 us a step, where the matrix instructions alone would take
+// 0.45 and 0.11.  4096 x 16384 x 8192 on random rows 306 us, 3.6 PFLOP/s.  E4M3: the matrix instructions, of which the split makes
+// two, at 70 to 80 % of their rate: 602 to 650 us, 1.7 to 1.8 PFLOP/s.
 // Two steps a stage (128 bytes of every row, one stage ahead) are 2 to 5 % faster for 256 x 256 of E2M1: on random rows
 // 4096 x 16384 x 8192 306 us, 316 with one, 4096 x 8192 x 2048 52, 54.6; for the smaller tiles, whose waves have nobody to
 // take turns with, 10 to 20 % slower.
@@ -515,17 +516,25 @@ static int mm_rows_launch(const MmArgs &a, const char *who, int rm = 16, int rn 
 // has at most one workgroup (a step's latency), `full` for 256 workgroups of a launch that fills the card many times over;
 // tiles are alike, so they come in whole rounds of 256 (2738 x 1951 x 9540 E4M3, 352 tiles of 128 x 128 147 us, 688 of 64 x 128
 // 123).
-// Measured at K = 8192, in microseconds, E4M3 / E2M1:
+// Measured at K = 8192, in microseconds, E4M3 / E2M1, on random rows, three sets of operands in turn (of 32768 rows of B more
+// than the last cache holds: 33 us are what memory takes for them), at clocks at which the first is 4 % slower than at best:
 //                        256x256      128x128     64x128      64x64       16x64       16x32       16x16
-//   4096 x 16384        631 / 272    860 / 373   947 / 517  1032 / 716
-//   4096 x 1024         135 /  61     74 /  34    63 /  37    73 /  48
-//   1024 x 1024         133 /  59     72 /  32    43 /  23    30 /  18
-//    256 x 1024                                   42 /  22    29 /  18    18 /  14    21 /  16    27 /  19
-//     64 x 1024                                   42 /  22    29 /  18    18 /  14    12 /   9     9 /   7
-//     16 x 32768                                  45 /  24    43 /  24    31 /  26    38 /  31    52 / -
-//      1 x 32768                                  45 /  24    42 /  23    28 /  24    30 /  28    33 / 32
-//      1 x 16384                                  42 /  22    29 /  19    17 /  16    18 /  17    19 / 17
-//      1 x 8192                                   41 /  22    29 /  18    16 /  13    11 /   8     9 / -
+//   4096 x 16384        650 / 322    894 / 439   983 / 588  1091 / 753
+//   4096 x 4096         159 /  83    228 / 110   255 / 148   276 / 194
+//   2048 x 2048         135 /  67     78 /  37    68 /  42    75 /  55
+//   1024 x 1024         132 /  65     74 /  34    45 /  24    32 /  20    57 / 47     70 / 56
+//    256 x 1024         134 /  65     73 /  33    45 /  23    31 /  19    19 / 15     22 / 17     29 / 21
+//     64 x 1024         133 /  64     72 /  32    44 /  23    31 /  19    19 / 14     13 / 10     10 /  7
+//     16 x 32768        142 /  70     76 /  42    48 /  37    45 /  37    38 / 33     43 / 36     54 / 40
+//      1 x 32768        135 /  69     74 /  41    47 /  36    45 /  35    34 / 30     35 / 31     34 / 30
+//      1 x 16384        133 /  64     71 /  33    45 /  23    32 /  20    18 / 16     18 / 17     18 / 16
+//      1 x 8192         133 /  64     71 /  32    45 /  23    31 /  19    17 / 14     13 / 11     11 / 10
+// The costs below are of one set of operands, which the last cache holds, and for E2M1 not of random ones: the table's
+// times lie 2 to 18 % above them, the large tiles' most, and where memory bounds all kinds by up to half.  The choice
+// stands: of 90 random sizes up to 8192 x 32768 x 16384, timed as the table was with every kind that comes near, it was within
+// 2 % of the fastest on 78 and within 12 % on 87; the farthest 1 x 20876 x 702 E4M3, 7.7 us where tiles of 16 x 32 take 5.5.  256 x
+// 256: a round of up to 64 tiles takes 2.1 / 1.04 us a step, of 256 tiles 2.49 / 1.30; its `full` stands for either, and
+// `alone` is 0.
 // The last kind's time goes with the row pieces that its loads touch, (E4M3: 8, E2M1: 4) + 1 per row of A and 5 per row of B
 // in four steps; where its tiles do not give every CU one, they are made of fewer rows (8 or 4 of the 16) on the side
 // that costs least: 1001 x 10 x 16384 E4M3 13.3 us with whole tiles, 10.2 with 8 rows, 8.8 with 4; 16 x 1000 x 32768 E2M1
@@ -536,10 +545,10 @@ struct MmCost {
 };
 constexpr MmCost kMmCosts[2][6] = {
     // E2M1 x E2M1
-    {{256, 256, 0.92, 1.07}, {128, 128, 0.50, 0.364}, {64, 128, 0.34, 0.253}, {64, 64, 0.27, 0.173},
+    {{256, 256, 0.0, 1.07}, {128, 128, 0.50, 0.364}, {64, 128, 0.34, 0.253}, {64, 64, 0.27, 0.173},
      {16, 64, 0.20, 0.18}, {16, 32, 0.11, 0.105}},
     // E4M3 x E2M1
-    {{256, 256, 2.1, 2.46}, {128, 128, 1.15, 0.88}, {64, 128, 0.62, 0.469}, {64, 64, 0.45, 0.261},
+    {{256, 256, 0.0, 2.46}, {128, 128, 1.15, 0.88}, {64, 128, 0.62, 0.469}, {64, 64, 0.45, 0.261},
      {16, 64, 0.25, 0.22}, {16, 32, 0.15, 0.14}},
 };
 

@@ -9,11 +9,15 @@
 // ones: one kernel over chunks of 8192 entries (the exponentials, which bound the whole, are then spread over the card
 // however few the rows), one workgroup per row to finish from the chunks' histograms.
 //
-// What bounds it: rows of up to 16376 entries and few rows of any length, the latency of about ten phases that follow each
-// other (a phase 1 to 4 us, most of it waiting for one workgroup's instructions and for memory); 256 x 131072 bf16 with a
-// cut, 93 us: 48 us the exponentials' kernel (37 instructions an entry, two thirds of the cycles), 45 us the rows' kernel, 10
-// of them the second look at every logit at what the last cache gives to all CUs (7 TB/s).  A border's bin of more entries
-// than the list holds costs a pass over the row per digit: 4 x 131072 equal logits 518 us, of N(0, 0.001^2) 298 us.
+// What bounds it: few rows, the latency of about ten phases that follow each other (a phase 1 to 4 us, most of it waiting for
+// one workgroup's instructions and for memory).  Rows of 65 to 16376 entries that outnumber what the card holds, instructions:
+// 4000 x 8000 bf16 without a cut 69 us, with top_p 165, where the bytes would take 13; an entry's weight is made once for the
+// histogram and once for the draw, its bin by a chain of its own, and registers spill: to 128 (four waves a SIMD) 38 to 43
+// vector registers of the forms with four groups a thread (156 to 176 bytes a lane), 7 to 10 of those with two, 7 and 17 to 18
+// of the long rows' kernel with 512 and 1024 threads; none with one group.  256 x 131072 bf16 with a cut, 93 us: 48 us the
+// exponentials' kernel (37 instructions an entry, two thirds of the cycles), 45 us the rows' kernel, 10 of them the second look
+// at every logit at what the last cache gives to all CUs (7 TB/s).  A border's bin of more entries than the list holds costs a
+// pass over the row per digit: 4 x 131072 equal logits 518 us, of N(0, 0.001^2) 298 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -1230,6 +1234,8 @@ static int token_launch(const TokenArgs &a, hipStream_t st, const char *who)
     //   8,  512, 4000 x 4000 bf16      17, 23, 148 /  20, 24, 101
     //   8,  512, 4000 x 8000 bf16      24, 34, 219 /  31, 36, 165
     //  10,      1024 x 16000 fp32      29,     115 /  31,      83
+    // fp32 and int32 have the same borders: at one the form for few rows takes as long as the other or up to 4 us less, a row above
+    // it up to 10 us more (with top_p 512 rows of 8000 fp32 34 / 36, 513 46 / 40; 256 of 16000 int32 37 / 39, 257 55 / 45).
     // By chunks: 64 x 32768 bf16 17 / 31, 5 x 50001 fp16 17 / 32, 256 x 131072 bf16 51 / 93, the largest entry alone 20.  512
     // threads a row, 1024 for the longest: 1024 x 32768 bf16 113, 160; 400 x 131072 161, 155; 1 x 131072 fp32 43, 37.
     const auto launch = [&](auto *kernel, int threads) { kernel<<<dim3((unsigned)a.R), dim3(threads), 0, st>>>(a); };

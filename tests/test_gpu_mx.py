@@ -214,8 +214,8 @@ def test_product(ops, shape, a_format):
             assert np.all(np.abs(got - want) <= bound * (1 + half))
 
 
-# sizes at which each of the kernels is the cheapest (tiles of 256x256, 128x128, 64x128, 64x64; 16 rows by 64, 32, 16), K of one
-# step, of whole groups of four steps and of odd ones
+# larger sizes (which tile a size takes goes by the format too: see TILES for a list that has every tile of both), K of one step, of
+# whole groups of four steps and of odd ones
 LARGE = [(8100, 8191, 1100), (8192, 8192, 128), (8000, 8300, 512), (3000, 3000, 700), (2048, 2100, 1536), (2049, 2100, 200),
          (2000, 1100, 900), (1030, 1025, 2048), (1000, 1000, 1000), (20, 33000, 640), (7, 40000, 1150), (40, 8000, 3000),
          (1, 3000, 6000), (2000, 20, 2100), (3, 129, 33000)]
