@@ -566,8 +566,8 @@ int64_t nb_mx_mm_tile(int64_t M, int64_t N, int64_t K, int A_format);
  * 16376 entries of the largest of about 8192 neighbours, so some are finer), so sums do not depend on an order of work;
  * weights below half a unit of that are never drawn.
  * temperature, top_k, top_p, min_p: per-row arrays [R], or NULL for the value that follows each of them for all rows
- * (not NaN).  NaN in an array: the row's largest entry (temperature), nothing cut (top_p, min_p).  1 <= V <= 2^20; any
- * number of rows.  workspace: nb_sample_tokens_workspace_bytes(R, V) bytes, 16-byte aligned (NULL if 0).
+ * (not NaN).  NaN in an array: the row's largest entry (temperature), nothing cut (top_p, min_p).  1 <= V <= 2^20,
+ * R <= 2^40 (in as many launches as it takes).  workspace: nb_sample_tokens_workspace_bytes(R, V) bytes, 16-byte aligned (NULL if 0).
  *   stands beside nb_sample_from_words (a bit per threshold and word); no counterpart in the reference. */
 int64_t nb_sample_tokens_workspace_bytes(int64_t R, int64_t V);
 int nb_sample_tokens(int32_t *out, const void *logits, int type, const uint32_t *words, const float *temperature,

@@ -555,7 +555,7 @@ constexpr MmCost kMmCosts[2][6] = {
 struct MmPlan {
     int kind, rm, rn;     // rm, rn: rows of A and B in a tile
 };
-// Tiles of one launch: its threads are counted in 32 bits, by kinds of 8 waves (the first, the last) and of 4.
+// Tiles of one launch: 2^31 threads of the staged kinds, below 2^32 of the others; the first and the last kind have 8 waves, the rest 4.
 constexpr double kMmMost[7] = {1 << 22, 1 << 23, 1 << 23, 1 << 23, (1 << 24) - 1, (1 << 24) - 1, (1 << 23) - 1};
 
 static MmPlan mm_plan(int64_t M, int64_t N, int64_t steps, bool fp8)
